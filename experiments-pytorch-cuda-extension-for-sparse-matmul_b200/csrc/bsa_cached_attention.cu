@@ -1,0 +1,759 @@
+// Attention of drafted tokens over a paged key / value cache (sm_100a only):
+//   o_i = sum_j p_ij v_j,   p_ij = exp(scale q_i k_j - lse_i)   over the keys j that draft i sees:
+// every cached token before the sequence's drafts, and among the drafts those whose bit is set in word i of `tree`
+// (none given: the drafts up to i itself).  A block layout, where given, takes away the keys of the blocks it lacks.
+//
+// One token of a sequence is a handful of query rows (drafts x the heads that share a key head), so the work is the
+// cache read once: bound by DRAM from a few thousand cached tokens on, below that by the two launches.
+//
+// Split.  The unit is a tile of 64 keys of one (sequence, key head, row tile); the units of the whole batch are one list,
+// and 2 x #SM persistent CTAs take equal contiguous shares of it, whatever the lengths are: nothing about the lengths is
+// known on the host.  A CTA that holds all tiles of a (sequence, head) writes its output; the others leave (O, m, l) in
+// fp32, at most two per CTA, and a second small kernel joins them in the order of the tiles (no atomics: the result does
+// not depend on timing).
+//
+// A CTA is a producer warp (TMA boxes of the pages, swizzled, into a ring of stages; one lane per page of the tile) and
+// four warps that each take 16 * G of the 64 keys for 16 of the 16 * G rows (G = 1, 2, 4 row groups): with few rows every
+// stored byte is read from shared memory once.  Products are m16n8k16 with the operands where ldmatrix leaves them:
+// at these row counts the tensor pipe idles either way, and a 128-row tcgen05 tile would be 7/8 padding.
+//
+// e4m3 caches.  Codes are exact in fp16, so the products run in fp16 on the codes themselves and the scales go where they
+// are cheap: the key's into the score, and the value's into the weight: with y_ij = log2(e) scale q_i k_j + log2 sv_j the
+// weights are P_ij = 2^(y_ij - m_i), m_i the running maximum of y (so P <= 1 whatever the scales are), O += P code,
+// l += P / sv_j, o = O / l.  bf16 queries are brought to fp16 by a power of two per row (exact but for values below
+// 2^-14 of the row's largest).  The 8-bit elements are paired by ldmatrix as 16-bit units, which permutes the
+// contraction axis of Q K^T (the query is loaded in the same order) and the columns of O (undone at the store).
+//
+// P is rounded to the products' 16-bit type (relative 2^-9 in bf16, 2^-12 in fp16), l, m and O are fp32.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "bsa_tc_common.cuh"
+
+namespace bsa {
+namespace {
+
+constexpr int kTileKeys = 64;
+constexpr int kConsumers = 4;                   // warps
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct CachedParams {
+    const void* q;
+    void* o;
+    int64_t q_batch, q_draft, q_head;           // strides of q in elements
+    const float* scales[2];
+    const int32_t* table;
+    const int32_t* lengths;
+    const int32_t* counts;                      // may be null
+    const int64_t* tree;                        // may be null
+    const uint8_t* pattern;                     // may be null: [pattern_rows, pattern_cols] of 1 << pattern_shift tokens
+    int pattern_rows, pattern_cols, pattern_shift;
+    int batch, drafts, group, kv_heads, row_tiles, table_width, pages, page_shift;
+    float scale_log2;                           // scale * log2 e
+    float* partial;                             // [ctas][2][rows][head_dim], then [ctas][2][rows][2] of (m, l)
+    int ctas;
+    uint32_t* status;
+};
+
+struct Share {
+    int64_t per, first, end;        // units per CTA; this CTA's range
+    int b, hm, tile;                // where the range starts
+};
+
+template <int kStages>
+struct __align__(8) CachedBarriers {
+    uint64_t full[kStages], empty[kStages];
+    uint32_t ok[kStages];           // bit i: page i of the stage's tile was loaded
+    Share share;
+    int abort_flag;
+};
+
+__device__ __forceinline__ int cached_length(const CachedParams& p, int b) {
+    return min(max(p.lengths[b], 0), p.table_width << p.page_shift);
+}
+__device__ __forceinline__ int cached_tiles(const CachedParams& p, int b) {
+    return max(1, (cached_length(p, b) + kTileKeys - 1) / kTileKeys);
+}
+
+// Sum of all tiles (of one head and row tile) of the batch, by one warp.
+__device__ __forceinline__ int64_t total_tiles(const CachedParams& p, int lane) {
+    int64_t sum = 0;
+    for (int b = lane; b < p.batch; b += 32) sum += cached_tiles(p, b);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    return sum;
+}
+// Tiles of the sequences before b, by one warp.
+__device__ __forceinline__ int64_t tiles_before(const CachedParams& p, int b_end, int lane) {
+    int64_t sum = 0;
+    for (int b = lane; b < b_end; b += 32) sum += cached_tiles(p, b);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    return sum;
+}
+
+__device__ __forceinline__ Share find_share(const CachedParams& p, int cta, int lane) {
+    Share s;
+    const int hms = p.kv_heads * p.row_tiles;
+    const int64_t units = total_tiles(p, lane) * hms;
+    s.per = (units + p.ctas - 1) / p.ctas;
+    s.first = min((int64_t)cta * s.per, units);
+    s.end = min(s.first + s.per, units);
+    s.b = s.hm = s.tile = 0;
+    if (s.first >= s.end) return s;
+    int64_t before = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+        const int mine = b0 + lane < p.batch ? cached_tiles(p, b0 + lane) : 0;
+        int64_t upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t o = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += o;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, s.first < (before + upto) * hms);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            const int tiles = __shfl_sync(0xffffffffu, mine, l);
+            const int64_t start = before + __shfl_sync(0xffffffffu, upto, l) - tiles;
+            const int64_t off = s.first - start * hms;
+            s.b = b0 + l;
+            s.hm = (int)(off / tiles);
+            s.tile = (int)(off - (int64_t)s.hm * tiles);
+            return s;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return s;
+}
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool kBf16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (kBf16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// two e4m3 codes (low 16 bits) as two fp16 values
+__device__ __forceinline__ uint32_t halves2(uint32_t codes) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3);
+    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+
+template <bool kE4m3, int kDim>
+struct CachedShape {
+    static constexpr int kRowBytes = kDim * (kE4m3 ? 1 : 2);
+    static constexpr int kPanelBytes = kRowBytes < 128 ? kRowBytes : 128;       // width of a TMA box
+    static constexpr int kPanels = kRowBytes / kPanelBytes;
+    static constexpr int kSideBytes = kTileKeys * kRowBytes;
+    static constexpr int kScaleBytes = kE4m3 ? 2 * kTileKeys * 4 : 0;
+    static constexpr int kStageBytes = 2 * kSideBytes;
+    // two CTAs per SM: 113 KB each, of which the merge buffers take up to 17
+    static constexpr int kStages = kStageBytes >= 32768 ? 3 : (kStageBytes >= 16384 ? 5 : 8);
+    static constexpr int kMergeBytes = 2 * 16 * kDim * 4 + 2 * 32 * 4 * 4;
+    static constexpr int kSmem = kStages * (kStageBytes + kScaleBytes) + kMergeBytes + (int)sizeof(CachedBarriers<kStages>);
+};
+// Byte offset of 16-byte chunk `chunk` of key `key` inside a side of a stage, as the TMA swizzle leaves it.
+template <bool kE4m3, int kDim>
+__device__ __forceinline__ uint32_t chunk_offset(int key, int chunk) {
+    using S = CachedShape<kE4m3, kDim>;
+    if (S::kPanelBytes == 128)
+        return (uint32_t)((chunk >> 3) * (kTileKeys * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
+    return (uint32_t)(key * 64 + ((chunk ^ ((key >> 1) & 3)) << 4));
+}
+
+// T: type of q and o; kGroups: groups of 16 rows (1, 2 or 4).
+template <typename T, bool kE4m3, int kDim, int kGroups>
+__global__ void __launch_bounds__((kConsumers + 1) * 32, 2)
+cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    using S = CachedShape<kE4m3, kDim>;
+    using Bars = CachedBarriers<S::kStages>;
+    constexpr bool kTBf16 = std::is_same_v<T, __nv_bfloat16>;
+    constexpr bool kBf16 = !kE4m3 && kTBf16;                // type of the products
+    constexpr int kRows = 16 * kGroups;
+    constexpr int kSplit = kConsumers / kGroups;            // warps that share a row group
+    constexpr int kWarpKeys = kTileKeys / kSplit;           // keys of a tile per warp
+    constexpr int kNT = kWarpKeys / 8;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* scale_smem = smem + S::kStages * S::kStageBytes;
+    float* merge = reinterpret_cast<float*>(scale_smem + S::kStages * S::kScaleBytes);
+    Bars* bars = reinterpret_cast<Bars*>(reinterpret_cast<uint8_t*>(merge) + S::kMergeBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == 0) {
+        const Share mine = find_share(p, (int)blockIdx.x, lane);
+        if (lane == 0) bars->share = mine;
+    } else if (warp == kConsumers && lane == 0) {
+        bars->abort_flag = 0;
+        for (int i = 0; i < S::kStages; ++i) {
+            mbar_init(&bars->full[i], 1);
+            mbar_init(&bars->empty[i], kConsumers);
+        }
+        fence_async_shared();
+    }
+    __syncthreads();
+    const Share share = bars->share;
+    int b = share.b, hm = share.hm, tile = share.tile;
+    const int hms = p.kv_heads * p.row_tiles;
+    int stage = 0;
+    uint32_t phase = 0;
+
+    if (warp == kConsumers) {                               // ---- producer
+        const int page = 1 << p.page_shift, piece = min(page, kTileKeys), pieces = kTileKeys / piece;
+        int length = 0, tiles = 0, at_b = -1;
+        bool dead = false;
+        for (int64_t u = share.first; u < share.end && !dead; ++u) {
+            if (b != at_b) {
+                at_b = b;
+                length = cached_length(p, b);
+                tiles = max(1, (length + kTileKeys - 1) / kTileKeys);
+                if (lane == 0 && p.lengths[b] != length) atomicExch(p.status, (uint32_t)BSA_ERR_BAD_SHAPE);
+            }
+            const int head = hm / p.row_tiles;
+            const int key = tile * kTileKeys + lane * piece;
+            bool ok = lane < pieces && key < length;
+            int row = 0;
+            if (ok) {
+                const int id = p.table[(int64_t)b * p.table_width + (key >> p.page_shift)];
+                if ((uint32_t)id >= (uint32_t)p.pages) {    // not a page of this cache: its keys are left out, and reported
+                    atomicExch(p.status, (uint32_t)BSA_ERR_BAD_SHAPE);
+                    ok = false;
+                } else {
+                    row = ((id * p.kv_heads + head) << p.page_shift) + (key & (page - 1));
+                }
+            }
+            const uint32_t loaded = __ballot_sync(0xffffffffu, ok);
+            dead = !mbar_wait(&bars->empty[stage], phase ^ 1, &bars->abort_flag, p.status);
+            if (dead) break;
+            if (lane == 0) {
+                bars->ok[stage] = loaded;
+                mbar_expect_tx(&bars->full[stage], (uint32_t)(__popc(loaded) * piece * (2 * S::kRowBytes + (kE4m3 ? 8 : 0))));
+            }
+            __syncwarp();
+            if (ok) {
+                uint8_t* base = smem + stage * S::kStageBytes;
+#pragma unroll
+                for (int side = 0; side < 2; ++side) {
+                    const CUtensorMap* map = side == 0 ? &map_k : &map_v;
+#pragma unroll
+                    for (int panel = 0; panel < S::kPanels; ++panel)
+                        tma_load_3d(base + side * S::kSideBytes + panel * (kTileKeys * S::kPanelBytes) + lane * piece * S::kPanelBytes,
+                                    map, &bars->full[stage], panel * (S::kPanelBytes / (kE4m3 ? 1 : 2)), row, 0);
+                    if (kE4m3)
+                        bulk_load_1d(scale_smem + stage * S::kScaleBytes + side * (kTileKeys * 4) + lane * piece * 4,
+                                     p.scales[side] + row, (uint32_t)(piece * 4), &bars->full[stage]);
+                }
+            }
+            if (++stage == S::kStages) { stage = 0; phase ^= 1; }
+            if (++tile == tiles) {
+                tile = 0;
+                if (++hm == hms) { hm = 0; ++b; }
+            }
+        }
+        if (dead) let_copies_land();
+        return;
+    }
+
+    // ---- consumers
+    const int rg = warp / kSplit, part = warp % kSplit;     // row group; which keys of a tile
+    const int g = lane >> 2, c = lane & 3;
+    bool dead = false;
+    int64_t u = share.first;
+    while (u < share.end) {
+        const int length = cached_length(p, b), tiles = max(1, (length + kTileKeys - 1) / kTileKeys);
+        const int count = p.counts ? min(max(p.counts[b], 0), p.drafts) : p.drafts;
+        const int prefix = length - count;                  // negative where a sequence has fewer tokens than drafts
+        const int head = hm / p.row_tiles, row_tile = hm - head * p.row_tiles;
+        const int todo = (int)min((int64_t)(tiles - tile), share.end - u);
+        const bool whole = tile == 0 && todo == tiles;
+        const bool from_start = tile == 0;
+
+        // this thread's two rows
+        uint64_t sees[2];
+        int row_block[2];
+        bool live[2];
+        int64_t q_at[2], o_at[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = row_tile * kRows + rg * 16 + g + 8 * r;
+            const int draft = row / p.group, of_group = row - draft * p.group;
+            live[r] = draft < p.drafts;
+            const int h = head * p.group + of_group;
+            q_at[r] = b * p.q_batch + draft * p.q_draft + h * p.q_head;
+            o_at[r] = (((int64_t)b * p.drafts + draft) * (p.kv_heads * p.group) + h) * kDim;
+            sees[r] = 0;
+            row_block[r] = -1;
+            if (live[r] && draft < count) {
+                sees[r] = p.tree ? (uint64_t)p.tree[(int64_t)b * p.drafts + draft] : ~0ull >> (63 - draft);
+                // a draft stands behind the prefix and its ancestors: its depth is the number of those
+                if (p.pattern) row_block[r] = (max(prefix, 0) + max(__popcll(sees[r]) - 1, 0)) >> p.pattern_shift;
+            }
+        }
+        const bool row_on[2] = {live[0] && (row_tile * kRows + rg * 16 + g) / p.group < count,
+                                live[1] && (row_tile * kRows + rg * 16 + g + 8) / p.group < count};
+
+        // query fragments
+        uint32_t qf[kDim / 16][4];
+        float row_scale[2] = {p.scale_log2, p.scale_log2};
+        if (!kE4m3) {
+#pragma unroll
+            for (int s = 0; s < kDim / 16; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = e & 1;
+                    qf[s][e] = row_on[r] ? *reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + q_at[r] + 16 * s + 2 * c + 8 * (e >> 1)) : 0u;
+                }
+        } else {
+            uint2 raw[kDim / 16][2];
+            uint32_t top[2] = {0, 0};
+#pragma unroll
+            for (int s = 0; s < kDim / 16; ++s)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    raw[s][r] = row_on[r] ? *reinterpret_cast<const uint2*>(static_cast<const T*>(p.q) + q_at[r] + 16 * s + 4 * c) : make_uint2(0u, 0u);
+                    const T* x = reinterpret_cast<const T*>(&raw[s][r]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top[r] = max(top[r], __float_as_uint(Scalar<T>::to_float(x[e])) & 0x7fffffffu);
+                }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float down = 1.0f;
+                if (kTBf16) {
+                    top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                    top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                    const int e = min(max((int)(top[r] >> 23), 1), 253);         // biased exponent of the row's largest
+                    down = __uint_as_float((uint32_t)(254 - e) << 23);            // 2^-(e - 127)
+                    row_scale[r] = p.scale_log2 * __uint_as_float((uint32_t)e << 23);
+                }
+#pragma unroll
+                for (int s = 0; s < kDim / 16; ++s) {
+                    const T* x = reinterpret_cast<const T*>(&raw[s][r]);
+                    qf[s][r] = pack2<false>(Scalar<T>::to_float(x[0]) * down, Scalar<T>::to_float(x[1]) * down);
+                    qf[s][2 + r] = pack2<false>(Scalar<T>::to_float(x[2]) * down, Scalar<T>::to_float(x[3]) * down);
+                }
+            }
+        }
+
+        float out[kDim / 8][4];
+#pragma unroll
+        for (int i = 0; i < kDim / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[i][e] = 0.0f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+        for (int i = 0; i < todo; ++i, ++tile) {
+            if (!dead) dead = !mbar_wait(&bars->full[stage], phase, &bars->abort_flag, p.status);
+            const uint32_t k_base = smem_u32(smem) + stage * S::kStageBytes, v_base = k_base + S::kSideBytes;
+            const uint32_t loaded = bars->ok[stage];
+            const int key0 = tile * kTileKeys + part * kWarpKeys;
+            float s[kNT][4];
+#pragma unroll
+            for (int n = 0; n < kNT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+            // Q K^T
+#pragma unroll
+            for (int n = 0; n < kNT; ++n) {
+                const int key = part * kWarpKeys + n * 8 + (lane & 7);
+                if (!kE4m3) {
+#pragma unroll
+                    for (int x = 0; x < kDim / 32; ++x) {
+                        uint32_t kf[4];
+                        ldsm_x4(k_base + chunk_offset<kE4m3, kDim>(key, 4 * x + (lane >> 3)), kf);
+                        mma_16816<kBf16>(s[n], qf[2 * x], kf[0], kf[1]);
+                        mma_16816<kBf16>(s[n], qf[2 * x + 1], kf[2], kf[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < kDim / 64; ++x) {
+                        uint32_t kf[4];
+                        ldsm_x4(k_base + chunk_offset<kE4m3, kDim>(key, 4 * x + (lane >> 3)), kf);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mma_16816<false>(s[n], qf[4 * x + e], halves2(kf[e]), halves2(kf[e] >> 16));
+                    }
+                }
+            }
+            // scores in units of log2; for e4m3 with the value's scale in the weight
+            const float* scales = reinterpret_cast<const float*>(scale_smem + stage * S::kScaleBytes) + part * kWarpKeys + 2 * c;
+            float inv[kNT][2];
+#pragma unroll
+            for (int n = 0; n < kNT; ++n) {
+                if (kE4m3) {
+                    const float2 sk = *reinterpret_cast<const float2*>(scales + n * 8);
+                    const float2 sv = *reinterpret_cast<const float2*>(scales + kTileKeys + n * 8);
+                    const float lv[2] = {__log2f(sv.x), __log2f(sv.y)};
+                    inv[n][0] = __frcp_rn(sv.x);
+                    inv[n][1] = __frcp_rn(sv.y);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[n][e] = fmaf(s[n][e] * ((e & 1) ? sk.y : sk.x), row_scale[e >> 1], lv[e & 1]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n][e] *= row_scale[e >> 1];
+                }
+            }
+            const int tile_end = (tile + 1) * kTileKeys;
+            const bool all_loaded = loaded == (1u << (kTileKeys >> min(p.page_shift, 6))) - 1u;
+            const bool masked = tile_end > prefix || !all_loaded || p.pattern != nullptr;
+            uint32_t keep[kNT];                             // per n-tile: which of this thread's two keys are really there
+            if (masked) {
+                const int piece_shift = min(p.page_shift, 6);
+#pragma unroll
+                for (int n = 0; n < kNT; ++n) {
+                    keep[n] = 0;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int key = key0 + n * 8 + 2 * c + e, draft = key - prefix;
+                        const bool there = key < length && (loaded >> ((key & (kTileKeys - 1)) >> piece_shift) & 1u);
+                        if (there) keep[n] |= e ? 0xffff0000u : 0x0000ffffu;
+                        int key_block = -1;
+                        if (p.pattern && there) {
+                            int place = key;
+                            if (draft >= 0) {
+                                const uint64_t w = p.tree ? (uint64_t)p.tree[(int64_t)b * p.drafts + draft] : ~0ull >> (63 - draft);
+                                place = max(prefix, 0) + max(__popcll(w) - 1, 0);
+                            }
+                            key_block = place >> p.pattern_shift;
+                        }
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            bool seen = there && row_on[r] && (draft < 0 || (sees[r] >> draft & 1ull));
+                            if (p.pattern && seen)
+                                seen = row_block[r] < p.pattern_rows && key_block < p.pattern_cols &&
+                                       p.pattern[(int64_t)row_block[r] * p.pattern_cols + key_block] != 0;
+                            if (!seen) s[n][2 * r + e] = -INFINITY;
+                        }
+                        if (kE4m3 && !there) inv[n][e] = 0.0f;
+                    }
+                }
+            }
+            // running maximum
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int n = 0; n < kNT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+            float ref[2];
+            bool raise = false;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                raise |= top[r] > m[r];
+            }
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float higher = fmaxf(m[r], top[r]);
+                    const float fall = higher == -INFINITY ? 1.0f : attn_exp2(m[r] - higher);
+                    m[r] = higher;
+                    l[r] *= fall;
+#pragma unroll
+                    for (int d = 0; d < kDim / 8; ++d) {
+                        out[d][2 * r] *= fall;
+                        out[d][2 * r + 1] *= fall;
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) ref[r] = m[r] == -INFINITY ? 0.0f : m[r];
+#pragma unroll
+            for (int n = 0; n < kNT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[n][e] = attn_exp2(s[n][e] - ref[e >> 1]);
+                    l[e >> 1] += kE4m3 ? s[n][e] * inv[n][e & 1] : s[n][e];
+                }
+            // P V
+#pragma unroll
+            for (int ks = 0; ks < kWarpKeys / 16; ++ks) {
+                const uint32_t pf[4] = {pack2<kBf16>(s[2 * ks][0], s[2 * ks][1]), pack2<kBf16>(s[2 * ks][2], s[2 * ks][3]),
+                                        pack2<kBf16>(s[2 * ks + 1][0], s[2 * ks + 1][1]), pack2<kBf16>(s[2 * ks + 1][2], s[2 * ks + 1][3])};
+                // lanes 0-7: keys 0-7 of the step, chunk a; 8-15: keys 8-15, chunk a; 16-31: the same of chunk a + 1
+                const int key = part * kWarpKeys + ks * 16 + (lane & 15);
+#pragma unroll
+                for (int a = 0; a < S::kRowBytes / 16; a += 2) {
+                    uint32_t vf[4];
+                    ldsm_x4_trans(v_base + chunk_offset<kE4m3, kDim>(key, a + (lane >> 4)), vf);
+                    if (masked) {                           // what is not there may be anything, a NaN too
+                        vf[0] &= keep[2 * ks]; vf[1] &= keep[2 * ks + 1];
+                        vf[2] &= keep[2 * ks]; vf[3] &= keep[2 * ks + 1];
+                    }
+                    if (!kE4m3) {
+                        mma_16816<kBf16>(out[a], pf, vf[0], vf[1]);
+                        mma_16816<kBf16>(out[a + 1], pf, vf[2], vf[3]);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {       // bytes (0, 2): even columns of the chunk, (1, 3): odd ones
+                            const uint32_t w0 = __byte_perm(vf[2 * x], 0, 0x3120), w1 = __byte_perm(vf[2 * x + 1], 0, 0x3120);
+                            mma_16816<false>(out[2 * (a + x)], pf, halves2(w0), halves2(w1));
+                            mma_16816<false>(out[2 * (a + x) + 1], pf, halves2(w0 >> 16), halves2(w1 >> 16));
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->empty[stage]);
+            if (++stage == S::kStages) { stage = 0; phase ^= 1; }
+        }
+        // the quad's four partial sums of a row
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        }
+        // the warps that share a row group: the upper half hands its (O, m, l) to the lower until one is left
+#pragma unroll
+        for (int half = kSplit / 2; half > 0; half >>= 1) {
+            const int buffer = kGroups == 1 ? part % half : rg % 2;
+            float* mo = merge + buffer * (16 * kDim);
+            float* ml = merge + 2 * 16 * kDim + buffer * 128;
+            if (part >= half && part < 2 * half) {
+#pragma unroll
+                for (int d = 0; d < kDim / 8; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mo[(d * 4 + e) * 32 + lane] = out[d][e];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) { ml[r * 32 + lane] = m[r]; ml[64 + r * 32 + lane] = l[r]; }
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
+            if (part < half) {
+                float mine[2], theirs[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float om = ml[r * 32 + lane], higher = fmaxf(m[r], om);
+                    const float ref = higher == -INFINITY ? 0.0f : higher;
+                    mine[r] = attn_exp2(m[r] - ref);
+                    theirs[r] = attn_exp2(om - ref);
+                    l[r] = l[r] * mine[r] + ml[64 + r * 32 + lane] * theirs[r];
+                    m[r] = higher;
+                }
+#pragma unroll
+                for (int d = 0; d < kDim / 8; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) out[d][e] = out[d][e] * mine[e >> 1] + mo[(d * 4 + e) * 32 + lane] * theirs[e >> 1];
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
+        }
+        if (part == 0) {
+            const int slot = from_start ? 1 : 0;
+            const int64_t part_row = ((int64_t)blockIdx.x * 2 + slot) * kRows + rg * 16 + g;
+            float* ml = p.partial + (int64_t)p.ctas * 2 * kRows * kDim;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                if (!live[r]) continue;
+                const bool any = row_on[r] && l[r] != 0.0f;          // false: the row sees nothing, and is zero whatever V holds
+                const float by = !any ? 0.0f : (whole ? 1.0f / l[r] : 1.0f);
+                if (!whole && c == 0) {
+                    ml[(part_row + 8 * r) * 2] = any ? m[r] : -INFINITY;
+                    ml[(part_row + 8 * r) * 2 + 1] = any ? l[r] : 0.0f;
+                }
+#pragma unroll
+                for (int d = 0; d < kDim / 8; d += (kE4m3 ? 2 : 1)) {
+                    // e4m3: tiles d, d + 1 hold the even and odd columns of chunk d / 2, this thread's are 4 c .. 4 c + 3
+                    const int col = kE4m3 ? 8 * d + 4 * c : 8 * d + 2 * c;
+                    float x[4];
+                    x[0] = out[d][2 * r];
+                    x[1] = kE4m3 ? out[kE4m3 ? d + 1 : d][2 * r] : out[d][2 * r + 1];
+                    x[2] = out[d][2 * r + 1];
+                    x[3] = out[kE4m3 ? d + 1 : d][2 * r + 1];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = any ? x[e] * by : 0.0f;
+                    if (whole) {
+                        T* to = static_cast<T*>(p.o) + o_at[r] + col;
+                        if (kE4m3) {
+                            uint2 w;
+                            w.x = pack2<kTBf16>(x[0], x[1]);
+                            w.y = pack2<kTBf16>(x[2], x[3]);
+                            *reinterpret_cast<uint2*>(to) = w;
+                        } else {
+                            *reinterpret_cast<uint32_t*>(to) = pack2<kTBf16>(x[0], x[1]);
+                        }
+                    } else {
+                        float* to = p.partial + (part_row + 8 * r) * kDim + col;
+                        if (kE4m3) *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+                        else *reinterpret_cast<float2*>(to) = make_float2(x[0], x[1]);
+                    }
+                }
+            }
+        }
+        u += todo;
+        if (tile == tiles) {
+            tile = 0;
+            if (++hm == hms) { hm = 0; ++b; }
+        }
+    }
+}
+
+// Joins what several CTAs left of one (sequence, key head, row tile): one warp per row, kDim / 32 columns per lane.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(128)
+cached_join_kernel(const CachedParams p, int rows) {
+    __shared__ int64_t shared[2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int hms = p.kv_heads * p.row_tiles, b = blockIdx.x / hms, hm = blockIdx.x - b * hms;
+    if (warp == 0) {
+        const int64_t all = total_tiles(p, lane), before = tiles_before(p, b, lane);
+        if (lane == 0) { shared[0] = all; shared[1] = before; }
+    }
+    __syncthreads();
+    const int64_t per = (shared[0] * hms + p.ctas - 1) / p.ctas;
+    const int tiles = cached_tiles(p, b);
+    const int64_t start = shared[1] * hms + (int64_t)hm * tiles, end = start + tiles;
+    const int first = (int)(start / per), last = (int)((end - 1) / per);
+    if (first == last) return;                              // one CTA had all of it and wrote the output
+    const int head = hm / p.row_tiles, row_tile = hm - head * p.row_tiles;
+    const float* ml = p.partial + (int64_t)p.ctas * 2 * rows * kDim;
+    constexpr int kCols = kDim / 32;
+    for (int r = warp; r < rows; r += 4) {
+        const int row = row_tile * rows + r, draft = row / p.group;
+        if (draft >= p.drafts) break;
+        float top = -INFINITY;
+        for (int i = first + lane; i <= last; i += 32) {
+            const int slot = (int64_t)i * per > start ? 0 : 1;
+            top = fmaxf(top, ml[(((int64_t)i * 2 + slot) * rows + r) * 2]);
+        }
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float sum[kCols], l = 0.0f;
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) sum[e] = 0.0f;
+#pragma unroll 4
+        for (int i = first; i <= last; ++i) {
+            const int slot = (int64_t)i * per > start ? 0 : 1;
+            const int64_t at = ((int64_t)i * 2 + slot) * rows + r;
+            const float2 w = *reinterpret_cast<const float2*>(ml + at * 2);
+            const float weight = attn_exp2(w.x - ref);
+            l += w.y * weight;
+            const float* x = p.partial + at * kDim + lane * kCols;      // (zeros where this part saw nothing)
+#pragma unroll
+            for (int e = 0; e < kCols; ++e) sum[e] += x[e] * weight;
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        T* to = static_cast<T*>(p.o) + (((int64_t)b * p.drafts + draft) * (p.kv_heads * p.group) + head * p.group + (row - draft * p.group)) * kDim + lane * kCols;
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) to[e] = Scalar<T>::from_float(sum[e] * inv);
+    }
+}
+
+// Map of a side of the cache as rows of head_dim elements, one page (at most a tile of it) per box.
+bool make_cache_map(CUtensorMap* map, int store, int dtype, const void* base, int64_t rows, int64_t dim, int piece) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const int es = store == BSA_CACHE_E4M3 ? 1 : 2, row_bytes = (int)dim * es, panel = row_bytes < 128 ? row_bytes : 128;
+    const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)rows, 1};
+    const cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)row_bytes * (cuuint64_t)rows};
+    const cuuint32_t box[3] = {(cuuint32_t)(panel / es), (cuuint32_t)piece, 1};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    const CUtensorMapDataType type = es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                             : (dtype == BSA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
+    return fn(map, type, 3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              panel == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int row_groups(int64_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
+
+template <typename T, bool kE4m3, int kDim, int kGroups>
+int launch_cached(const CachedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t stream) {
+    auto kernel = cached_attention_kernel<T, kE4m3, kDim, kGroups>;
+    constexpr int smem = CachedShape<kE4m3, kDim>::kSmem;
+    if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return BSA_ERR_LAUNCH;
+    kernel<<<p.ctas, (kConsumers + 1) * 32, smem, stream>>>(p, map_k, map_v);
+    cached_join_kernel<T, kDim><<<p.batch * p.kv_heads * p.row_tiles, 128, 0, stream>>>(p, 16 * kGroups);
+    return launch_status();
+}
+template <typename T, bool kE4m3, int kDim>
+int launch_groups(int groups, const CachedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t stream) {
+    if (groups == 1) return launch_cached<T, kE4m3, kDim, 1>(p, map_k, map_v, stream);
+    if (groups == 2) return launch_cached<T, kE4m3, kDim, 2>(p, map_k, map_v, stream);
+    return launch_cached<T, kE4m3, kDim, 4>(p, map_k, map_v, stream);
+}
+template <typename T>
+int launch_cached_typed(int store, int64_t dim, int groups, const CachedParams& p, const CUtensorMap& map_k,
+                        const CUtensorMap& map_v, cudaStream_t stream) {
+    if (store == BSA_CACHE_E4M3)
+        return dim == 64 ? launch_groups<T, true, 64>(groups, p, map_k, map_v, stream)
+                         : launch_groups<T, true, 128>(groups, p, map_k, map_v, stream);
+    return dim == 64 ? launch_groups<T, false, 64>(groups, p, map_k, map_v, stream)
+                     : launch_groups<T, false, 128>(groups, p, map_k, map_v, stream);
+}
+
+}  // namespace
+}  // namespace bsa
+
+extern "C" size_t bsa_cached_attention_scratch(int64_t drafts, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
+    if (drafts <= 0 || kv_heads <= 0 || q_heads < kv_heads || head_dim <= 0) return 0;
+    const int sms = bsa::sm_count();
+    return (size_t)std::max(sms, 1) * 2 * 2 * 16 * bsa::row_groups(drafts * (q_heads / kv_heads)) * (size_t)(head_dim + 2) * 4;
+}
+
+extern "C" int bsa_cached_attention(int dtype, int store, const void* q, int64_t q_batch_stride, int64_t q_draft_stride,
+                                    int64_t q_head_stride, const void* keys, const void* values, const float* key_scales,
+                                    const float* value_scales, void* o, const int32_t* table, const int32_t* lengths,
+                                    const int32_t* counts, const int64_t* tree, const uint8_t* pattern,
+                                    int64_t pattern_rows, int64_t pattern_cols, int64_t pattern_block, int64_t batch,
+                                    int64_t drafts, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t pages,
+                                    int64_t page, int64_t table_width, float scale, void* scratch, size_t scratch_bytes,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace bsa;
+    const int checked = check_cache(dtype, store, key_scales, value_scales, pages, kv_heads, page, head_dim);
+    if (checked != BSA_OK) return checked;
+    if (batch < 0 || drafts <= 0 || q_heads <= 0 || q_heads % kv_heads != 0 || table_width <= 0) return BSA_ERR_BAD_SHAPE;
+    if (drafts > 64) return BSA_ERR_TOO_LARGE;              // one bit of a tree word per draft
+    if (!workspace || workspace_bytes < BSA_WORKSPACE_BYTES) return BSA_ERR_WORKSPACE;
+    if (pattern && (!valid_block((int)pattern_block) || pattern_block > 128)) return BSA_ERR_BAD_BLOCK;
+    if (pattern && (pattern_rows <= 0 || pattern_cols <= 0 || pattern_rows > 65535 || pattern_cols > 65535)) return BSA_ERR_BAD_SHAPE;
+    if (batch == 0) return BSA_OK;
+    if (!q || !keys || !values || !o || !table || !lengths || !scratch) return BSA_ERR_NULL_POINTER;
+    if (!aligned16(q) || !aligned16(keys) || !aligned16(values) || !aligned16(o) || !aligned16(scratch)) return BSA_ERR_ALIGNMENT;
+    if (store == BSA_CACHE_E4M3 && (!aligned16(key_scales) || !aligned16(value_scales))) return BSA_ERR_ALIGNMENT;
+    if (q_batch_stride < 0 || q_draft_stride < 0 || q_head_stride < 0) return BSA_ERR_BAD_SHAPE;
+    if (q_batch_stride % 8 || q_draft_stride % 8 || q_head_stride % 8) return BSA_ERR_ALIGNMENT;
+    if (table_width > (int64_t)(INT32_MAX - 256) / page) return BSA_ERR_TOO_LARGE;      // 32-bit positions in a sequence
+    CachedParams p{};
+    const int64_t group = q_heads / kv_heads;
+    const int groups = row_groups(drafts * group);
+    const int64_t row_tiles = (drafts * group + 16 * groups - 1) / (16 * groups);
+    if (row_tiles * kv_heads > (int64_t)INT32_MAX / batch || q_heads > 65535) return BSA_ERR_TOO_LARGE;
+    p.q = q; p.o = o;
+    p.q_batch = q_batch_stride; p.q_draft = q_draft_stride; p.q_head = q_head_stride;
+    p.scales[0] = key_scales; p.scales[1] = value_scales;
+    p.table = table; p.lengths = lengths; p.counts = counts; p.tree = tree;
+    p.pattern = pattern;
+    p.pattern_rows = (int)pattern_rows; p.pattern_cols = (int)pattern_cols;
+    while (pattern && (1 << p.pattern_shift) < pattern_block) ++p.pattern_shift;
+    p.batch = (int)batch; p.drafts = (int)drafts; p.group = (int)group; p.kv_heads = (int)kv_heads;
+    p.row_tiles = (int)row_tiles; p.table_width = (int)table_width; p.pages = (int)pages;
+    while ((1 << p.page_shift) < page) ++p.page_shift;
+    p.scale_log2 = scale * kLog2e;
+    p.partial = static_cast<float*>(scratch);
+    p.ctas = 2 * sm_count();
+    p.status = static_cast<uint32_t*>(workspace);
+    if (p.ctas <= 0) return BSA_ERR_LAUNCH;
+    if (scratch_bytes < bsa_cached_attention_scratch(drafts, q_heads, kv_heads, head_dim)) return BSA_ERR_WORKSPACE;
+    // the driver's encoder needs the device's context bound to this thread
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) { cudaGetLastError(); return BSA_ERR_LAUNCH; }
+    CUtensorMap map_k, map_v;
+    const int64_t rows = pages * kv_heads * page;
+    const int piece = (int)std::min<int64_t>(page, kTileKeys);
+    if (!make_cache_map(&map_k, store, dtype, keys, rows, head_dim, piece) ||
+        !make_cache_map(&map_v, store, dtype, values, rows, head_dim, piece)) return BSA_ERR_DRIVER;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return dtype == BSA_DTYPE_F16 ? launch_cached_typed<__half>(store, head_dim, groups, p, map_k, map_v, s)
+                                  : launch_cached_typed<__nv_bfloat16>(store, head_dim, groups, p, map_k, map_v, s);
+}

@@ -393,6 +393,146 @@ torch::Tensor sparse_to_dense(torch::Tensor x, torch::Tensor row_blocks, int64_t
     return convert(false, x, row_blocks, rows, cols, block);
 }
 
+// A paged cache as the bindings see it: [pages, heads, page, head_dim] twice, and for e4m3 the scales [pages, heads, page].
+struct Cache {
+    int dtype, store;
+    int64_t pages, heads, page, dim;
+    float* key_scales = nullptr;
+    float* value_scales = nullptr;
+};
+
+Cache check_cache(const torch::Tensor& keys, const torch::Tensor& values, const c10::optional<torch::Tensor>& key_scales,
+                  const c10::optional<torch::Tensor>& value_scales, at::ScalarType dtype, const torch::Device& device) {
+    TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "the tokens must be float16 or bfloat16, got ", dtype);
+    TORCH_CHECK(keys.device() == device && values.device() == device && device.is_cuda(),
+                "tokens and cache must be CUDA tensors on one device");
+    TORCH_CHECK(keys.dim() == 4 && keys.sizes() == values.sizes(), "keys and values must share a shape [pages, heads, page, head_dim]");
+    TORCH_CHECK(keys.is_contiguous() && values.is_contiguous(), "keys and values must be contiguous");
+    TORCH_CHECK(keys.scalar_type() == values.scalar_type(), "keys and values must have the same dtype");
+    Cache c;
+    c.dtype = dtype == at::kHalf ? BSA_DTYPE_F16 : BSA_DTYPE_BF16;
+    c.pages = keys.size(0); c.heads = keys.size(1); c.page = keys.size(2); c.dim = keys.size(3);
+    TORCH_CHECK(c.page == 16 || c.page == 32 || c.page == 64 || c.page == 128, "page size must be 16, 32, 64 or 128, got ", c.page);
+    TORCH_CHECK(c.dim == 64 || c.dim == 128, "head_dim must be 64 or 128, got ", c.dim);
+    const bool scaled = key_scales.has_value() && key_scales->defined();
+    TORCH_CHECK(scaled == (value_scales.has_value() && value_scales->defined()), "give the scales of both keys and values, or of neither");
+    if (keys.scalar_type() == at::kFloat8_e4m3fn) {
+        TORCH_CHECK(scaled, "a float8_e4m3fn cache needs key_scales and value_scales");
+        c.store = BSA_CACHE_E4M3;
+        for (const auto* s : {&*key_scales, &*value_scales}) {
+            TORCH_CHECK(s->scalar_type() == at::kFloat && s->device() == device && s->is_contiguous() &&
+                        s->sizes() == keys.sizes().slice(0, 3), "scales must be contiguous float32 [pages, heads, page]");
+        }
+        c.key_scales = key_scales->data_ptr<float>();
+        c.value_scales = value_scales->data_ptr<float>();
+    } else {
+        TORCH_CHECK(keys.scalar_type() == dtype, "the cache must hold the tokens' dtype or float8_e4m3fn");
+        TORCH_CHECK(!scaled, "scales belong to a float8_e4m3fn cache");
+        c.store = BSA_CACHE_SAME;
+    }
+    return c;
+}
+
+// `x` as the kernels read it: last axis contiguous, 16-byte aligned rows (a copy where it is laid out otherwise, as the
+// other ops make their operands contiguous).
+torch::Tensor row_aligned(torch::Tensor x) {
+    bool ok = x.stride(-1) == 1 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+    for (int64_t i = 0; ok && i + 1 < x.dim(); ++i) ok = x.size(i) == 1 || x.stride(i) % 8 == 0;
+    return ok ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+// stride of an axis (an axis of one element may carry any stride: read as 0)
+int64_t axis_stride(const torch::Tensor& x, int64_t i) { return x.size(i) == 1 ? 0 : x.stride(i); }
+
+void check_slots(const torch::Tensor& slots, const torch::Device& device) {
+    TORCH_CHECK(slots.dim() == 1 && slots.scalar_type() == at::kLong && slots.device() == device && slots.is_contiguous(),
+                "slots must be a contiguous int64 tensor [tokens] on the cache's device");
+}
+
+// Keys and values of new tokens into the paged cache, in place.
+void cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torch::Tensor keys, torch::Tensor values,
+                 c10::optional<torch::Tensor> key_scales, c10::optional<torch::Tensor> value_scales) {
+    TORCH_CHECK(k.dim() == 3 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() && k.device() == v.device(),
+                "k and v must share a shape [tokens, heads, head_dim], dtype and device");
+    const Cache c = check_cache(keys, values, key_scales, value_scales, k.scalar_type(), k.device());
+    check_slots(slots, k.device());
+    TORCH_CHECK(k.size(1) == c.heads && k.size(2) == c.dim, "k and v must be [tokens, ", c.heads, ", ", c.dim, "] for this cache");
+    TORCH_CHECK(slots.size(0) == k.size(0), "slots holds ", slots.size(0), " entries, k ", k.size(0), " tokens");
+    if (k.size(0) == 0) return;
+    c10::cuda::CUDAGuard guard(k.device());
+    k = row_aligned(k);
+    v = row_aligned(v);
+    auto ws = workspace_for(k.device());
+    check_status(bsa_cache_write(c.dtype, c.store, k.data_ptr(), v.data_ptr(), axis_stride(k, 0), axis_stride(k, 1),
+                                 axis_stride(v, 0), axis_stride(v, 1), slots.data_ptr<int64_t>(), k.size(0),
+                                 keys.data_ptr(), values.data_ptr(), c.key_scales, c.value_scales, c.pages, c.heads,
+                                 c.page, c.dim, ws.data_ptr(), BSA_WORKSPACE_BYTES,
+                                 at::cuda::getCurrentCUDAStream().stream()), "cache_write");
+}
+
+// (k, v) [tokens, heads, head_dim] of the given slots as 16-bit values.
+std::tuple<torch::Tensor, torch::Tensor> cache_read(torch::Tensor slots, torch::Tensor keys, torch::Tensor values,
+                                                    c10::optional<torch::Tensor> key_scales,
+                                                    c10::optional<torch::Tensor> value_scales, at::ScalarType dtype) {
+    const Cache c = check_cache(keys, values, key_scales, value_scales, dtype, keys.device());
+    check_slots(slots, keys.device());
+    c10::cuda::CUDAGuard guard(keys.device());
+    auto k = torch::empty({slots.size(0), c.heads, c.dim}, keys.options().dtype(dtype));
+    auto v = torch::empty_like(k);
+    if (slots.size(0) > 0) {
+        auto ws = workspace_for(keys.device());
+        check_status(bsa_cache_read(c.dtype, c.store, slots.data_ptr<int64_t>(), slots.size(0), keys.data_ptr(),
+                                    values.data_ptr(), c.key_scales, c.value_scales, k.data_ptr(), v.data_ptr(), c.pages,
+                                    c.heads, c.page, c.dim, ws.data_ptr(), BSA_WORKSPACE_BYTES,
+                                    at::cuda::getCurrentCUDAStream().stream()), "cache_read");
+    }
+    return {k, v};
+}
+
+// Attention of q [batch, drafts, q_heads, head_dim] over a paged cache.
+torch::Tensor cached_attention(torch::Tensor q, torch::Tensor keys, torch::Tensor values,
+                               c10::optional<torch::Tensor> key_scales, c10::optional<torch::Tensor> value_scales,
+                               torch::Tensor table, torch::Tensor lengths, c10::optional<torch::Tensor> counts,
+                               c10::optional<torch::Tensor> tree, double scale, c10::optional<torch::Tensor> pattern,
+                               int64_t pattern_block) {
+    TORCH_CHECK(q.dim() == 4, "q must be [batch, drafts, heads, head_dim]");
+    const Cache c = check_cache(keys, values, key_scales, value_scales, q.scalar_type(), q.device());
+    const int64_t batch = q.size(0), drafts = q.size(1), heads = q.size(2);
+    TORCH_CHECK(q.size(3) == c.dim, "q has head_dim ", q.size(3), ", the cache ", c.dim);
+    TORCH_CHECK(heads > 0 && heads % c.heads == 0, "the ", heads, " query heads must be a multiple of the cache's ", c.heads);
+    TORCH_CHECK(drafts >= 1 && drafts <= 64, "1 to 64 drafts per sequence, got ", drafts);
+    const auto check_ints = [&](const torch::Tensor& t, at::ScalarType type, at::IntArrayRef sizes, const char* what) {
+        TORCH_CHECK(t.scalar_type() == type && t.device() == q.device() && t.is_contiguous() && t.sizes() == sizes, what);
+    };
+    TORCH_CHECK(table.dim() == 2 && table.size(0) == batch && table.size(1) > 0 && table.scalar_type() == at::kInt &&
+                table.device() == q.device() && table.is_contiguous(), "table must be a contiguous int32 tensor [batch, pages] on q's device");
+    check_ints(lengths, at::kInt, {batch}, "lengths must be a contiguous int32 tensor [batch] on q's device");
+    if (counts.has_value() && counts->defined())
+        check_ints(*counts, at::kInt, {batch}, "counts must be a contiguous int32 tensor [batch] on q's device");
+    if (tree.has_value() && tree->defined())
+        check_ints(*tree, at::kLong, {batch, drafts}, "tree must be a contiguous int64 tensor [batch, drafts] on q's device");
+    const bool patterned = pattern.has_value() && pattern->defined();
+    if (patterned)
+        TORCH_CHECK(pattern->dim() == 2 && pattern->scalar_type() == at::kByte && pattern->device() == q.device() &&
+                    pattern->is_contiguous(), "pattern must be a contiguous uint8 tensor [block rows, block columns] on q's device");
+    c10::cuda::CUDAGuard guard(q.device());
+    auto o = torch::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+    if (batch == 0) return o;
+    q = row_aligned(q);
+    auto ws = workspace_for(q.device());
+    const size_t bytes = bsa_cached_attention_scratch(drafts, heads, c.heads, c.dim);
+    auto scratch = torch::empty({static_cast<int64_t>(bytes)}, q.options().dtype(torch::kUInt8));
+    check_status(bsa_cached_attention(
+        c.dtype, c.store, q.data_ptr(), axis_stride(q, 0), axis_stride(q, 1), axis_stride(q, 2), keys.data_ptr(),
+        values.data_ptr(), c.key_scales, c.value_scales, o.data_ptr(), table.data_ptr<int>(), lengths.data_ptr<int>(),
+        counts.has_value() && counts->defined() ? counts->data_ptr<int>() : nullptr,
+        tree.has_value() && tree->defined() ? tree->data_ptr<int64_t>() : nullptr,
+        patterned ? pattern->data_ptr<uint8_t>() : nullptr, patterned ? pattern->size(0) : 0, patterned ? pattern->size(1) : 0,
+        pattern_block, batch, drafts, heads, c.heads, c.dim, c.pages, c.page, table.size(1), static_cast<float>(scale),
+        scratch.data_ptr(), bytes, ws.data_ptr(), BSA_WORKSPACE_BYTES, at::cuda::getCurrentCUDAStream().stream()),
+        "cached_attention");
+    return o;
+}
+
 // The ops of this module never synchronise; a kernel that gives up on a bounded wait, or meets a
 // block descriptor that does not belong to its layout, leaves a status in the module's per-device
 // workspace instead.  check_device_status(device_index) synchronises the current stream of that
@@ -433,6 +573,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("build_layout", &build_layout, "Build row / column layout metadata on the device.", py::arg("pattern"));
     m.def("dense_to_sparse", &dense_to_sparse, "Gather the layout's blocks from a dense matrix.");
     m.def("sparse_to_dense", &sparse_to_dense, "Scatter blocks into a zero-filled dense matrix.");
+    m.def("cache_write", &cache_write, "Write tokens' keys and values into a paged cache.", py::arg("k"), py::arg("v"),
+          py::arg("slots"), py::arg("keys"), py::arg("values"), py::arg("key_scales") = py::none(),
+          py::arg("value_scales") = py::none());
+    m.def("cache_read", &cache_read, "Keys and values of the given slots of a paged cache.", py::arg("slots"),
+          py::arg("keys"), py::arg("values"), py::arg("key_scales"), py::arg("value_scales"), py::arg("dtype"));
+    m.def("cached_attention", &cached_attention, "Attention of drafted tokens over a paged cache.", py::arg("q"),
+          py::arg("keys"), py::arg("values"), py::arg("key_scales"), py::arg("value_scales"), py::arg("table"),
+          py::arg("lengths"), py::arg("counts") = py::none(), py::arg("tree") = py::none(), py::arg("scale") = 1.0,
+          py::arg("pattern") = py::none(), py::arg("pattern_block") = 0);
     m.def("check_device_status", &check_device_status, "Synchronise the device's current stream; raise if a kernel reported a time-out or a bad block descriptor since the last check.",
           py::arg("device_index") = 0);
     m.def("version", []() { return bsa_version(); });

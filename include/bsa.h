@@ -40,7 +40,7 @@ enum {
     BSA_ERR_BAD_DTYPE = 3,      /* dtype code unknown or unsupported here     */
     BSA_ERR_BAD_SHAPE = 4,      /* a size is negative, zero where it must not
                                    be, or not a multiple of the block size    */
-    BSA_ERR_BAD_BLOCK = 5,      /* block size is not 16, 32, 64 or 128        */
+    BSA_ERR_BAD_BLOCK = 5,      /* block (page) size is not 16, 32, 64 or 128 */
     BSA_ERR_ALIGNMENT = 6,      /* a pointer is not 16-byte aligned           */
     BSA_ERR_WORKSPACE = 7,      /* workspace missing or too small             */
     BSA_ERR_LAUNCH = 8,         /* the CUDA runtime refused the launch        */
@@ -57,6 +57,8 @@ enum { BSA_DTYPE_F32 = 0, BSA_DTYPE_F16 = 1, BSA_DTYPE_BF16 = 2 };
 enum { BSA_PATTERN_U8 = 0, BSA_PATTERN_I32 = 1, BSA_PATTERN_I64 = 2, BSA_PATTERN_F32 = 3 };
 /* which kernel family bsa_matmul uses */
 enum { BSA_ENGINE_AUTO = 0, BSA_ENGINE_SIMT = 1, BSA_ENGINE_TCGEN05 = 2 };
+/* how a key / value cache holds its numbers: the tokens' own 16-bit type, or e4m3 with fp32 scales */
+enum { BSA_CACHE_SAME = 0, BSA_CACHE_E4M3 = 1 };
 
 /* bytes of device workspace every matmul call needs (zero it once after
  * allocation; the library keeps it zero between successful calls) */
@@ -224,6 +226,79 @@ int bsa_attention_backward(int dtype, const void* q, const void* k, const void* 
                            int quadrant_masks,
                            void* stats, size_t stats_bytes,
                            void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Paged key / value cache: write the keys and values of new tokens, read places back.
+ * No counterpart in the reference (it has no cached inference).
+ *
+ *   dtype           BSA_DTYPE_F16 / BSA_DTYPE_BF16: type of the tokens (k, v)
+ *   store           BSA_CACHE_SAME: the cache holds dtype; BSA_CACHE_E4M3: it holds
+ *                   e4m3 codes and one fp32 scale per token, head and side,
+ *                     a = max(max_d |x_d|, 2^-100), scale = a / 448,
+ *                     code_d = e4m3(x_d * (448 / a)), round to nearest even;
+ *                   a row with an infinity or NaN reads back as NaN
+ *   k, v            write: [tokens, heads, head_dim] with the given strides (in
+ *                   elements, multiples of 8; the last axis contiguous);
+ *                   read: contiguous output, 0 for skipped tokens
+ *   slots           device int64 [tokens]: page * page_size + place of every
+ *                   token; negative: skipped.  A slot behind the cache's end is
+ *                   skipped and reported (BSA_ERR_BAD_SHAPE in the workspace).
+ *                   The non-negative slots of one write must differ: two tokens
+ *                   written to one slot leave a row mixed from both.
+ *   keys, values    [pages, heads, page, head_dim], contiguous
+ *   key_scales,
+ *   value_scales    e4m3: float [pages, heads, page]; else ignored
+ * page 16, 32, 64 or 128; head_dim 64 or 128; pages * heads * page < 2^31.
+ */
+int bsa_cache_write(int dtype, int store, const void* k, const void* v, int64_t k_token_stride,
+                    int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots,
+                    int64_t tokens, void* keys, void* values, float* key_scales, float* value_scales,
+                    int64_t pages, int64_t heads, int64_t page, int64_t head_dim, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int bsa_cache_read(int dtype, int store, const int64_t* slots, int64_t tokens, const void* keys,
+                   const void* values, const float* key_scales, const float* value_scales, void* k, void* v,
+                   int64_t pages, int64_t heads, int64_t page, int64_t head_dim, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/*
+ * Attention of drafted tokens over the paged cache: draft i of sequence b sees
+ * the cached tokens before the sequence's drafts, and of those the ones whose
+ * bit is set in tree[b][i] (tree NULL: drafts 0 .. i, a chain).  One draft is
+ * ordinary decoding.  No counterpart in the reference.
+ *
+ *   q               [batch, drafts, q_heads, head_dim] with the given strides (in
+ *                   elements, multiples of 8; last axis contiguous); query head h
+ *                   reads key head h / (q_heads / kv_heads)
+ *   keys, values, key_scales, value_scales, pages, page, dtype, store
+ *                   the cache, as in bsa_cache_write
+ *   o               [batch, drafts, q_heads, head_dim], contiguous; drafts that see
+ *                   nothing, and those from counts[b] on, give 0
+ *   table           int32 [batch, table_width]: the pages of every sequence; only
+ *                   entries before its length are read.  An id outside [0, pages)
+ *                   leaves its keys out and is reported (BSA_ERR_BAD_SHAPE)
+ *   lengths         int32 [batch]: tokens of the sequence in the cache, its drafts
+ *                   (the last counts[b] of them) included; beyond table_width * page:
+ *                   cut off and reported
+ *   counts          int32 [batch] or NULL (every sequence has `drafts`)
+ *   tree            int64 [batch, drafts] or NULL
+ *   pattern         NULL, or uint8 [pattern_rows, pattern_cols]: key at position j is
+ *                   seen from position i only where
+ *                   pattern[i / pattern_block][j / pattern_block] is not 0 (positions
+ *                   outside the pattern see nothing).  A draft's position is the
+ *                   number of tokens before the drafts plus that of its ancestors.
+ *   scratch         bsa_cached_attention_scratch() bytes, 16-byte aligned, of this
+ *                   call alone until it is done
+ * drafts <= 64.
+ */
+size_t bsa_cached_attention_scratch(int64_t drafts, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
+int bsa_cached_attention(int dtype, int store, const void* q, int64_t q_batch_stride, int64_t q_draft_stride,
+                         int64_t q_head_stride, const void* keys, const void* values, const float* key_scales,
+                         const float* value_scales, void* o, const int32_t* table, const int32_t* lengths,
+                         const int32_t* counts, const int64_t* tree, const uint8_t* pattern,
+                         int64_t pattern_rows, int64_t pattern_cols, int64_t pattern_block, int64_t batch,
+                         int64_t drafts, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t pages,
+                         int64_t page, int64_t table_width, float scale, void* scratch, size_t scratch_bytes,
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Gather the blocks of a dense [batches, rows*block, cols*block] matrix into
