@@ -1,0 +1,166 @@
+// What the packed attention kernels share: finding a CTA's rows, 128-row operand tiles, TMEM accesses of one row per
+// thread, tensor maps over [tokens, heads, head_dim] with strides.
+#pragma once
+#include "bsa_tc_common.cuh"
+
+namespace bsa {
+namespace {
+
+constexpr int kRowsTile = 128;                              // query rows / keys of a tile: the M of an MMA
+constexpr int kPanelBytes = kRowsTile * 128;                // 128 rows x 64 elements of 16 bits, 128-byte swizzle
+constexpr float kPackedLog2e = 1.4426950408889634f;
+
+// One sequence's tile, or (b == batch) a tile of the rows behind the last sequence, which hold zeros.
+struct PackedItem {
+    int start, length, tile, b;                             // first row and rows of the sequence; length 0: nothing to do
+};
+
+// Item `rank` of the list of all tiles: the sequences in order, `per_tile` rows per tile, then the rows behind the last
+// sequence.  Called by one warp; nothing about the offsets is known on the host.  Offsets that are not
+// 0 <= o_0 = 0 <= o_1 <= .. <= rows are reported, and clamped so that nothing outside the tensors is touched.
+__device__ __forceinline__ PackedItem packed_locate(const int32_t* offsets, int batch, int rows, int per_tile, int rank,
+                                                    int lane, uint32_t* status) {
+    int before = 0;
+    for (int b0 = 0; b0 <= batch; b0 += 32) {
+        const int b = b0 + lane;
+        int start = 0, end = 0;
+        if (b <= batch) {
+            const int from = offsets[b], to = b < batch ? offsets[b + 1] : rows;
+            start = min(max(from, 0), rows);
+            end = min(max(to, start), rows);
+            if (from != start || to != end || (b == 0 && from != 0)) atomicExch(status, (uint32_t)BSA_ERR_BAD_SHAPE);
+        }
+        const int tiles = (end - start + per_tile - 1) / per_tile;
+        int upto = tiles;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += o;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, rank < before + upto);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            PackedItem item;
+            item.start = __shfl_sync(0xffffffffu, start, l);
+            item.length = __shfl_sync(0xffffffffu, end, l) - item.start;
+            item.tile = rank - before - __shfl_sync(0xffffffffu, upto - tiles, l);
+            item.b = b0 + l;
+            return item;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return PackedItem{0, 0, 0, 0};
+}
+
+// Operand descriptor of a 128-row tile in 64-element panels: K-major (a row is one M / N index) or MN-major (a row is
+// one K index; the leading offset is the distance of the panels, which hold consecutive 64-wide ranges of M / N).
+__device__ __forceinline__ uint64_t panel_desc(uint32_t smem_addr, bool mn_major) {
+    uint64_t d = (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(mn_major ? (kPanelBytes >> 4) : 1) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+// D[128 x 128] = A B^T over head_dim, both operands K-major in shared memory.
+template <int kDim>
+__device__ __forceinline__ void mma_rows(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc) {
+#pragma unroll
+    for (int kk = 0; kk < kDim / 16; ++kk) {
+        const uint64_t at = (uint64_t)((kk / 4) * (kPanelBytes >> 4) + (kk % 4) * 2);
+        tc_mma_f16(tmem_d, a + at, b + at, idesc, kk > 0 ? 1u : 0u);
+    }
+}
+// D[128 x head_dim] (+)= A B over 128 keys (rows), A in tensor memory as 16-bit pairs, B MN-major.
+__device__ __forceinline__ void mma_keys(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, bool accumulate) {
+#pragma unroll
+    for (int kk = 0; kk < kRowsTile / 16; ++kk)
+        tc_mma_f16_ts(tmem_d, tmem_a + (uint32_t)(8 * kk), b + (uint64_t)(kk * (2048 >> 4)), idesc, accumulate || kk > 0 ? 1u : 0u);
+}
+
+__device__ __forceinline__ void tc_st_32x32b_x32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+
+// Zeroes rows [from, 128) of a tile in shared memory (all lanes of a warp), for the tensor cores to read: what TMA
+// brought there belongs to another sequence, and 0 times a NaN of it would be NaN.
+template <int kDim>
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int lane) {
+#pragma unroll
+    for (int panel = 0; panel < kDim / 64; ++panel)
+        for (int at = from * 128 + lane * 16; at < kPanelBytes; at += 512)
+            *reinterpret_cast<uint4*>(tile + panel * kPanelBytes + at) = make_uint4(0u, 0u, 0u, 0u);
+    fence_async_shared();
+    __syncwarp();
+}
+
+// 32 fp32 values of a row, rounded, to global memory (64 bytes, 32-byte aligned).
+template <bool kBf16>
+__device__ __forceinline__ void store_row32(void* to, const uint32_t (&r)[32], float by) {
+    uint32_t w[8];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            w[i] = pack2<kBf16>(__uint_as_float(r[16 * half + 2 * i]) * by, __uint_as_float(r[16 * half + 2 * i + 1]) * by);
+        st_global_v8(static_cast<uint8_t*>(to) + 32 * half, w);
+    }
+}
+
+// Zero rows [from, to) of a contiguous 16-bit [rows, heads, head_dim] tensor, one head, by all threads of the CTA.
+__device__ __forceinline__ void zero_tail(void* base, int from, int to, int head, int heads, int dim) {
+    const int chunks = dim / 8;
+    for (int i = threadIdx.x; i < (to - from) * chunks; i += blockDim.x) {
+        const int row = from + i / chunks, c = i % chunks;
+        reinterpret_cast<uint4*>(base)[((size_t)row * heads + head) * chunks + c] = make_uint4(0u, 0u, 0u, 0u);
+    }
+}
+
+// Tensor map over [tokens, heads, head_dim] (16 bits, strides in elements): boxes of 64 elements x 1 head x 128 tokens.
+// Rows behind the last read as zero.
+bool make_packed_map(CUtensorMap* map, int dtype, const void* base, int64_t tokens, int64_t heads, int64_t dim,
+                     int64_t token_stride, int64_t head_stride) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
+    const cuuint32_t box[3] = {64, 1, kRowsTile};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    const CUtensorMapDataType type = dtype == BSA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return fn(map, type, 3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The driver's encoder needs the device's context bound to the calling thread.
+bool bind_device() {
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) return true;
+    cudaGetLastError();
+    return false;
+}
+
+// Argument checks of both directions; `tensors`: pointers that must be there and 16-byte aligned.
+int check_packed(int dtype, int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim) {
+    if (dtype != BSA_DTYPE_F16 && dtype != BSA_DTYPE_BF16) return BSA_ERR_BAD_DTYPE;
+    if (dim != 64 && dim != 128) return BSA_ERR_BAD_SHAPE;
+    if (rows < 0 || batch < 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads != 0) return BSA_ERR_BAD_SHAPE;
+    // 32-bit rows, tiles and CTA numbers
+    if (rows > (int64_t)INT32_MAX - 256 || batch > (1 << 24) || q_heads > 65535) return BSA_ERR_TOO_LARGE;
+    if ((rows / kRowsTile + batch + 2) * q_heads > (int64_t)INT32_MAX) return BSA_ERR_TOO_LARGE;
+    return BSA_OK;
+}
+int check_strides(int64_t token_stride, int64_t head_stride) {
+    if (token_stride <= 0 || head_stride <= 0 || token_stride >= (1ll << 38) || head_stride >= (1ll << 38)) return BSA_ERR_BAD_SHAPE;
+    return token_stride % 8 || head_stride % 8 ? BSA_ERR_ALIGNMENT : BSA_OK;
+}
+
+}  // namespace
+}  // namespace bsa

@@ -533,6 +533,76 @@ torch::Tensor cached_attention(torch::Tensor q, torch::Tensor keys, torch::Tenso
     return o;
 }
 
+// `x` [rows, heads, head_dim] as the packed kernels' tensor maps read it (a contiguous copy where it is laid out otherwise).
+torch::Tensor map_ready(torch::Tensor x) {
+    x = row_aligned(x);
+    for (int64_t i = 0; i < 2; ++i)
+        if (x.size(i) > 1 && x.stride(i) == 0) return x.contiguous();
+    return x;
+}
+int64_t map_stride(const torch::Tensor& x, int64_t i) { return x.size(i) == 1 ? x.size(1) * x.size(2) : x.stride(i); }
+
+void check_packed(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& offsets) {
+    TORCH_CHECK(q.is_cuda() && k.device() == q.device() && v.device() == q.device(), "q, k, v must be CUDA tensors on one device");
+    TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(2),
+                "q must be [rows, heads, head_dim], k and v [rows, kv_heads, head_dim]");
+    TORCH_CHECK(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type(), "q, k, v must share a dtype");
+    TORCH_CHECK(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16, "q, k, v must be float16 or bfloat16, got ", q.scalar_type());
+    TORCH_CHECK(q.size(2) == 64 || q.size(2) == 128, "head_dim must be 64 or 128, got ", q.size(2));
+    TORCH_CHECK(k.size(1) > 0 && q.size(1) > 0 && q.size(1) % k.size(1) == 0, "the ", q.size(1), " query heads must be a multiple of the ", k.size(1), " key heads");
+    TORCH_CHECK(offsets.dim() == 1 && offsets.size(0) >= 1 && offsets.scalar_type() == at::kInt && offsets.device() == q.device() &&
+                offsets.is_contiguous(), "offsets must be a contiguous int32 tensor [sequences + 1] on q's device");
+}
+
+// (o, lse) of attention inside the sequences of a packed batch; lse [heads, rows] in units of log2.
+std::tuple<torch::Tensor, torch::Tensor> packed_attention_forward(torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                                                                  torch::Tensor offsets, double scale, bool causal) {
+    check_packed(q, k, v, offsets);
+    c10::cuda::CUDAGuard guard(q.device());
+    auto o = torch::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+    auto lse = torch::empty({q.size(1), q.size(0)}, q.options().dtype(torch::kFloat));
+    if (q.size(0) > 0) {
+        q = map_ready(q); k = map_ready(k); v = map_ready(v);
+        auto ws = workspace_for(q.device());
+        check_status(bsa_packed_forward(dtype_code(q), q.data_ptr(), map_stride(q, 0), map_stride(q, 1), k.data_ptr(),
+                                        map_stride(k, 0), map_stride(k, 1), v.data_ptr(), map_stride(v, 0), map_stride(v, 1),
+                                        o.data_ptr(), lse.data_ptr<float>(), offsets.data_ptr<int>(), q.size(0),
+                                        offsets.size(0) - 1, q.size(1), k.size(1), q.size(2), static_cast<float>(scale), causal,
+                                        ws.data_ptr(), BSA_WORKSPACE_BYTES, at::cuda::getCurrentCUDAStream().stream()),
+                     "packed_attention_forward");
+    }
+    return {o, lse};
+}
+
+// (dq, dk, dv) from the inputs, the forward's results and the output's gradient.
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attention_backward(
+        torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor dout, torch::Tensor lse,
+        torch::Tensor offsets, double scale, bool causal) {
+    check_packed(q, k, v, offsets);
+    TORCH_CHECK(o.sizes() == q.sizes() && dout.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() &&
+                dout.scalar_type() == q.scalar_type() && o.device() == q.device() && dout.device() == q.device(),
+                "o and dout must have q's shape, dtype and device");
+    TORCH_CHECK(lse.scalar_type() == torch::kFloat && lse.is_contiguous() && lse.device() == q.device() && lse.dim() == 2 &&
+                lse.size(0) == q.size(1) && lse.size(1) == q.size(0), "lse must be the forward's, float32 [heads, rows]");
+    c10::cuda::CUDAGuard guard(q.device());
+    auto dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options()), dv = torch::empty(v.sizes(), v.options());
+    if (q.size(0) > 0) {
+        q = map_ready(q); k = map_ready(k); v = map_ready(v); dout = map_ready(dout);
+        o = o.contiguous();
+        auto ws = workspace_for(q.device());
+        auto stats = torch::empty({q.size(1), q.size(0), 2}, q.options().dtype(torch::kFloat));
+        check_status(bsa_packed_backward(dtype_code(q), q.data_ptr(), map_stride(q, 0), map_stride(q, 1), k.data_ptr(),
+                                         map_stride(k, 0), map_stride(k, 1), v.data_ptr(), map_stride(v, 0), map_stride(v, 1),
+                                         o.data_ptr(), dout.data_ptr(), map_stride(dout, 0), map_stride(dout, 1),
+                                         lse.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                         offsets.data_ptr<int>(), q.size(0), offsets.size(0) - 1, q.size(1), k.size(1), q.size(2),
+                                         static_cast<float>(scale), causal, stats.data_ptr(), static_cast<size_t>(stats.numel()) * 4,
+                                         ws.data_ptr(), BSA_WORKSPACE_BYTES, at::cuda::getCurrentCUDAStream().stream()),
+                     "packed_attention_backward");
+    }
+    return {dq, dk, dv};
+}
+
 // The ops of this module never synchronise; a kernel that gives up on a bounded wait, or meets a
 // block descriptor that does not belong to its layout, leaves a status in the module's per-device
 // workspace instead.  check_device_status(device_index) synchronises the current stream of that
@@ -582,6 +652,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("keys"), py::arg("values"), py::arg("key_scales"), py::arg("value_scales"), py::arg("table"),
           py::arg("lengths"), py::arg("counts") = py::none(), py::arg("tree") = py::none(), py::arg("scale") = 1.0,
           py::arg("pattern") = py::none(), py::arg("pattern_block") = 0);
+    m.def("packed_attention_forward", &packed_attention_forward,
+          "Attention inside the sequences of a packed batch; returns (output, log2-sum-exp).", py::arg("q"), py::arg("k"),
+          py::arg("v"), py::arg("offsets"), py::arg("scale") = 1.0, py::arg("causal") = true);
+    m.def("packed_attention_backward", &packed_attention_backward, "Its gradients (dq, dk, dv).", py::arg("q"), py::arg("k"),
+          py::arg("v"), py::arg("o"), py::arg("dout"), py::arg("lse"), py::arg("offsets"), py::arg("scale") = 1.0,
+          py::arg("causal") = true);
     m.def("check_device_status", &check_device_status, "Synchronise the device's current stream; raise if a kernel reported a time-out or a bad block descriptor since the last check.",
           py::arg("device_index") = 0);
     m.def("version", []() { return bsa_version(); });

@@ -228,6 +228,41 @@ int bsa_attention_backward(int dtype, const void* q, const void* k, const void* 
                            void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Attention inside the sequences of a packed batch, and its gradients.
+ * No counterpart in the reference (its operands are [..., seq, d] of one length).
+ *
+ *   q, dout, o, dq  [rows, q_heads, head_dim]; query head h reads key head
+ *                   h / (q_heads / kv_heads)
+ *   k, v, dk, dv    [rows, kv_heads, head_dim]
+ *                   inputs with the given strides (in elements, positive multiples
+ *                   of 8, the last axis contiguous, 16-byte aligned); outputs and o
+ *                   contiguous, 32-byte aligned
+ *   offsets         device int32 [batch + 1]: sequence b is the rows offsets[b] ..
+ *                   offsets[b + 1] - 1; offsets[0] = 0, not decreasing, at most
+ *                   `rows`.  Rows behind the last sequence get 0.  Other offsets are
+ *                   reported (BSA_ERR_BAD_SHAPE in the workspace) and touch nothing
+ *                   outside the tensors; the output is then not defined.
+ *   causal          nonzero: a row sees its own and earlier rows of its sequence
+ *   lse             float [q_heads, rows]: log2 of the row sums of
+ *                   exp(scale * s), -inf for rows behind the last sequence (forward:
+ *                   may be NULL)
+ *   stats           scratch of rows * q_heads * 8 bytes, 16-byte aligned
+ * BSA_DTYPE_F16 / BSA_DTYPE_BF16, head_dim 64 or 128.
+ */
+int bsa_packed_forward(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                       int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                       int64_t v_head_stride, void* o, float* lse, const int32_t* offsets, int64_t rows,
+                       int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scale, int causal,
+                       void* workspace, size_t workspace_bytes, void* stream);
+int bsa_packed_backward(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                        int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                        int64_t v_head_stride, const void* o, const void* dout, int64_t dout_token_stride,
+                        int64_t dout_head_stride, const float* lse, void* dq, void* dk, void* dv,
+                        const int32_t* offsets, int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                        int64_t head_dim, float scale, int causal, void* stats, size_t stats_bytes,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Paged key / value cache: write the keys and values of new tokens, read places back.
  * No counterpart in the reference (it has no cached inference).
  *
