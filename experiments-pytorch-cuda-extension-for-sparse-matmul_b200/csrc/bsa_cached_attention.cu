@@ -6,9 +6,9 @@
 // One token of a sequence is a handful of query rows (drafts x the heads that share a key head), so the work is the
 // cache read once: bound by DRAM from a few thousand cached tokens on, below that by the two launches.
 //
-// Split.  The unit is a tile of 64 keys of one (sequence, key head, row tile); the units of the whole batch are one list,
-// and 2 x #SM persistent CTAs take equal contiguous shares of it, whatever the lengths are: nothing about the lengths is
-// known on the host.  A CTA that holds all tiles of a (sequence, head) writes its output; the others leave (O, m, l) in
+// Split.  The unit is a tile of 64 keys of one (sequence, key head, row tile), and each of those begins with kBegin empty
+// units for what its first and last steps cost; the units of the whole batch are one list, and 2 x #SM persistent CTAs
+// take equal contiguous shares of it, whatever the lengths are: nothing about the lengths is known on the host.  A CTA that holds all tiles of a (sequence, head) writes its output; the others leave (O, m, l) in
 // fp32, at most two per CTA, and a second small kernel joins them in the order of the tiles (no atomics: the result does
 // not depend on timing).
 //
@@ -37,6 +37,7 @@ namespace {
 
 constexpr int kTileKeys = 64;
 constexpr int kConsumers = 4;                   // warps
+constexpr int kBegin = 3;                       // what beginning and ending a (sequence, head) costs a CTA, in tiles
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct CachedParams {
@@ -77,27 +78,31 @@ __device__ __forceinline__ int cached_tiles(const CachedParams& p, int b) {
     return max(1, (cached_length(p, b) + kTileKeys - 1) / kTileKeys);
 }
 
-// Sum of all tiles (of one head and row tile) of the batch, by one warp.
-__device__ __forceinline__ int64_t total_tiles(const CachedParams& p, int lane) {
-    int64_t sum = 0;
-    for (int b = lane; b < p.batch; b += 32) sum += cached_tiles(p, b);
+// Cost of one head and row tile of sequences 0 .. end - 1 (all of them before `part`, in `before`), by one warp.
+__device__ __forceinline__ int64_t total_cost(const CachedParams& p, int part, int64_t& before, int lane) {
+    int64_t sum = 0, some = 0;
+#pragma unroll 4
+    for (int b = lane; b < p.batch; b += 32) {
+        const int cost = cached_tiles(p, b) + kBegin;
+        sum += cost;
+        if (b < part) some += cost;
+    }
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-    return sum;
-}
-// Tiles of the sequences before b, by one warp.
-__device__ __forceinline__ int64_t tiles_before(const CachedParams& p, int b_end, int lane) {
-    int64_t sum = 0;
-    for (int b = lane; b < b_end; b += 32) sum += cached_tiles(p, b);
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    for (int s = 16; s > 0; s >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        some += __shfl_xor_sync(0xffffffffu, some, s);
+    }
+    before = some;
     return sum;
 }
 
+// A (sequence, head, row tile) takes kBegin + tiles units of the list, its tiles last.  Finds where this CTA's share
+// starts; a share that starts inside the first kBegin units starts at tile 0.
 __device__ __forceinline__ Share find_share(const CachedParams& p, int cta, int lane) {
     Share s;
     const int hms = p.kv_heads * p.row_tiles;
-    const int64_t units = total_tiles(p, lane) * hms;
+    int64_t none;
+    const int64_t units = total_cost(p, 0, none, lane) * hms;
     s.per = (units + p.ctas - 1) / p.ctas;
     s.first = min((int64_t)cta * s.per, units);
     s.end = min(s.first + s.per, units);
@@ -105,7 +110,7 @@ __device__ __forceinline__ Share find_share(const CachedParams& p, int cta, int 
     if (s.first >= s.end) return s;
     int64_t before = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
-        const int mine = b0 + lane < p.batch ? cached_tiles(p, b0 + lane) : 0;
+        const int mine = b0 + lane < p.batch ? cached_tiles(p, b0 + lane) + kBegin : 0;
         int64_t upto = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -115,12 +120,14 @@ __device__ __forceinline__ Share find_share(const CachedParams& p, int cta, int 
         const uint32_t past = __ballot_sync(0xffffffffu, s.first < (before + upto) * hms);
         if (past) {
             const int l = __ffs(past) - 1;
-            const int tiles = __shfl_sync(0xffffffffu, mine, l);
-            const int64_t start = before + __shfl_sync(0xffffffffu, upto, l) - tiles;
+            const int cost = __shfl_sync(0xffffffffu, mine, l);
+            const int64_t start = before + __shfl_sync(0xffffffffu, upto, l) - cost;
             const int64_t off = s.first - start * hms;
             s.b = b0 + l;
-            s.hm = (int)(off / tiles);
-            s.tile = (int)(off - (int64_t)s.hm * tiles);
+            s.hm = (int)(off / cost);
+            const int within = (int)(off - (int64_t)s.hm * cost);
+            s.tile = max(within - kBegin, 0);
+            s.first += max(kBegin - within, 0);             // the unit of that tile
             return s;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
@@ -186,7 +193,8 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
     constexpr int kRows = 16 * kGroups;
     constexpr int kSplit = kConsumers / kGroups;            // warps that share a row group
     constexpr int kWarpKeys = kTileKeys / kSplit;           // keys of a tile per warp
-    constexpr int kNT = kWarpKeys / 8;
+    constexpr int kStepKeys = kWarpKeys < 32 ? kWarpKeys : 32;          // keys of a step of the warp (registers)
+    constexpr int kNT = kStepKeys / 8;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* scale_smem = smem + S::kStages * S::kStageBytes;
     float* merge = reinterpret_cast<float*>(scale_smem + S::kStages * S::kScaleBytes);
@@ -212,28 +220,41 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
 
     if (warp == kConsumers) {                               // ---- producer
         const int page = 1 << p.page_shift, piece = min(page, kTileKeys), pieces = kTileKeys / piece;
-        int length = 0, tiles = 0, at_b = -1;
         bool dead = false;
-        for (int64_t u = share.first; u < share.end && !dead; ++u) {
-            if (b != at_b) {
-                at_b = b;
-                length = cached_length(p, b);
-                tiles = max(1, (length + kTileKeys - 1) / kTileKeys);
-                if (lane == 0 && p.lengths[b] != length) atomicExch(p.status, (uint32_t)BSA_ERR_BAD_SHAPE);
-            }
+        int64_t u = share.first;
+        int length = 0, tiles = 0, id = 0;
+        auto enter = [&]() {                                // a new sequence
+            length = cached_length(p, b);
+            tiles = max(1, (length + kTileKeys - 1) / kTileKeys);
+            if (lane == 0 && p.lengths[b] != length) atomicExch(p.status, (uint32_t)BSA_ERR_BAD_SHAPE);
+        };
+        auto look = [&]() {                                 // this lane's page of the tile
+            const int key = tile * kTileKeys + lane * piece;
+            id = 0;
+            if (lane < pieces && key < length) id = p.table[(int64_t)b * p.table_width + (key >> p.page_shift)];
+        };
+        if (u < share.end) { enter(); look(); }
+        while (u < share.end) {
             const int head = hm / p.row_tiles;
             const int key = tile * kTileKeys + lane * piece;
             bool ok = lane < pieces && key < length;
-            int row = 0;
-            if (ok) {
-                const int id = p.table[(int64_t)b * p.table_width + (key >> p.page_shift)];
-                if ((uint32_t)id >= (uint32_t)p.pages) {    // not a page of this cache: its keys are left out, and reported
-                    atomicExch(p.status, (uint32_t)BSA_ERR_BAD_SHAPE);
-                    ok = false;
-                } else {
-                    row = ((id * p.kv_heads + head) << p.page_shift) + (key & (page - 1));
+            if (ok && (uint32_t)id >= (uint32_t)p.pages) {  // not a page of this cache: its keys are left out, and reported
+                atomicExch(p.status, (uint32_t)BSA_ERR_BAD_SHAPE);
+                ok = false;
+            }
+            const int row = ok ? ((id * p.kv_heads + head) << p.page_shift) + (key & (page - 1)) : 0;
+            // on to the next tile: its page numbers travel while this one waits for its stage
+            ++u;
+            if (++tile == tiles) {
+                tile = 0;
+                u += kBegin;
+                if (++hm == hms) {
+                    hm = 0;
+                    ++b;
+                    if (u < share.end) enter();
                 }
             }
+            if (u < share.end) look();
             const uint32_t loaded = __ballot_sync(0xffffffffu, ok);
             dead = !mbar_wait(&bars->empty[stage], phase ^ 1, &bars->abort_flag, p.status);
             if (dead) break;
@@ -257,10 +278,6 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
                 }
             }
             if (++stage == S::kStages) { stage = 0; phase ^= 1; }
-            if (++tile == tiles) {
-                tile = 0;
-                if (++hm == hms) { hm = 0; ++b; }
-            }
         }
         if (dead) let_copies_land();
         return;
@@ -271,9 +288,14 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
     const int g = lane >> 2, c = lane & 3;
     bool dead = false;
     int64_t u = share.first;
+    int at_b = -1, length = 0, tiles = 0, count = 0;
     while (u < share.end) {
-        const int length = cached_length(p, b), tiles = max(1, (length + kTileKeys - 1) / kTileKeys);
-        const int count = p.counts ? min(max(p.counts[b], 0), p.drafts) : p.drafts;
+        if (b != at_b) {
+            at_b = b;
+            length = cached_length(p, b);
+            tiles = max(1, (length + kTileKeys - 1) / kTileKeys);
+            count = p.counts ? min(max(p.counts[b], 0), p.drafts) : p.drafts;
+        }
         const int prefix = length - count;                  // negative where a sequence has fewer tokens than drafts
         const int head = hm / p.row_tiles, row_tile = hm - head * p.row_tiles;
         const int todo = (int)min((int64_t)(tiles - tile), share.end - u);
@@ -357,7 +379,9 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             if (!dead) dead = !mbar_wait(&bars->full[stage], phase, &bars->abort_flag, p.status);
             const uint32_t k_base = smem_u32(smem) + stage * S::kStageBytes, v_base = k_base + S::kSideBytes;
             const uint32_t loaded = bars->ok[stage];
-            const int key0 = tile * kTileKeys + part * kWarpKeys;
+#pragma unroll 1
+            for (int base = part * kWarpKeys; base < (part + 1) * kWarpKeys; base += kStepKeys) {
+            const int key0 = tile * kTileKeys + base;
             float s[kNT][4];
 #pragma unroll
             for (int n = 0; n < kNT; ++n)
@@ -366,7 +390,7 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             // Q K^T
 #pragma unroll
             for (int n = 0; n < kNT; ++n) {
-                const int key = part * kWarpKeys + n * 8 + (lane & 7);
+                const int key = base + n * 8 + (lane & 7);
                 if (!kE4m3) {
 #pragma unroll
                     for (int x = 0; x < kDim / 32; ++x) {
@@ -386,7 +410,7 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
                 }
             }
             // scores in units of log2; for e4m3 with the value's scale in the weight
-            const float* scales = reinterpret_cast<const float*>(scale_smem + stage * S::kScaleBytes) + part * kWarpKeys + 2 * c;
+            const float* scales = reinterpret_cast<const float*>(scale_smem + stage * S::kScaleBytes) + base + 2 * c;
             float inv[kNT][2];
 #pragma unroll
             for (int n = 0; n < kNT; ++n) {
@@ -478,11 +502,11 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
                 }
             // P V
 #pragma unroll
-            for (int ks = 0; ks < kWarpKeys / 16; ++ks) {
+            for (int ks = 0; ks < kStepKeys / 16; ++ks) {
                 const uint32_t pf[4] = {pack2<kBf16>(s[2 * ks][0], s[2 * ks][1]), pack2<kBf16>(s[2 * ks][2], s[2 * ks][3]),
                                         pack2<kBf16>(s[2 * ks + 1][0], s[2 * ks + 1][1]), pack2<kBf16>(s[2 * ks + 1][2], s[2 * ks + 1][3])};
                 // lanes 0-7: keys 0-7 of the step, chunk a; 8-15: keys 8-15, chunk a; 16-31: the same of chunk a + 1
-                const int key = part * kWarpKeys + ks * 16 + (lane & 15);
+                const int key = base + ks * 16 + (lane & 15);
 #pragma unroll
                 for (int a = 0; a < S::kRowBytes / 16; a += 2) {
                     uint32_t vf[4];
@@ -503,6 +527,7 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
                         }
                     }
                 }
+            }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->empty[stage]);
@@ -592,6 +617,7 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
         u += todo;
         if (tile == tiles) {
             tile = 0;
+            u += kBegin;
             if (++hm == hms) { hm = 0; ++b; }
         }
     }
@@ -601,52 +627,45 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
 template <typename T, int kDim>
 __global__ void __launch_bounds__(128)
 cached_join_kernel(const CachedParams p, int rows) {
-    __shared__ int64_t shared[2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int hms = p.kv_heads * p.row_tiles, b = blockIdx.x / hms, hm = blockIdx.x - b * hms;
-    if (warp == 0) {
-        const int64_t all = total_tiles(p, lane), before = tiles_before(p, b, lane);
-        if (lane == 0) { shared[0] = all; shared[1] = before; }
-    }
-    __syncthreads();
-    const int64_t per = (shared[0] * hms + p.ctas - 1) / p.ctas;
+    const int hms = p.kv_heads * p.row_tiles;
+    const int in_tile = rows / 4, item = blockIdx.x / in_tile, r = (blockIdx.x - item * in_tile) * 4 + warp;
+    const int b = item / hms, hm = item - b * hms;
+    const int head = hm / p.row_tiles, row = (hm - head * p.row_tiles) * rows + r, draft = row / p.group;
+    if (draft >= p.drafts) return;
+    int64_t before;
+    const int64_t per = (total_cost(p, b, before, lane) * hms + p.ctas - 1) / p.ctas;
     const int tiles = cached_tiles(p, b);
-    const int64_t start = shared[1] * hms + (int64_t)hm * tiles, end = start + tiles;
-    const int first = (int)(start / per), last = (int)((end - 1) / per);
+    const int64_t start = before * hms + (int64_t)hm * (tiles + kBegin) + kBegin;       // the unit of tile 0
+    const int first = (int)(start / per), last = (int)((start + tiles - 1) / per);
     if (first == last) return;                              // one CTA had all of it and wrote the output
-    const int head = hm / p.row_tiles, row_tile = hm - head * p.row_tiles;
     const float* ml = p.partial + (int64_t)p.ctas * 2 * rows * kDim;
     constexpr int kCols = kDim / 32;
-    for (int r = warp; r < rows; r += 4) {
-        const int row = row_tile * rows + r, draft = row / p.group;
-        if (draft >= p.drafts) break;
-        float top = -INFINITY;
-        for (int i = first + lane; i <= last; i += 32) {
-            const int slot = (int64_t)i * per > start ? 0 : 1;
-            top = fmaxf(top, ml[(((int64_t)i * 2 + slot) * rows + r) * 2]);
-        }
+    float top = -INFINITY;
+    for (int i = first + lane; i <= last; i += 32) top = fmaxf(top, ml[(((int64_t)i * 2 + (i == first)) * rows + r) * 2]);
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-        const float ref = top == -INFINITY ? 0.0f : top;
-        float sum[kCols], l = 0.0f;
+    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum[kCols], l = 0.0f;
 #pragma unroll
-        for (int e = 0; e < kCols; ++e) sum[e] = 0.0f;
-#pragma unroll 4
-        for (int i = first; i <= last; ++i) {
-            const int slot = (int64_t)i * per > start ? 0 : 1;
-            const int64_t at = ((int64_t)i * 2 + slot) * rows + r;
-            const float2 w = *reinterpret_cast<const float2*>(ml + at * 2);
-            const float weight = attn_exp2(w.x - ref);
-            l += w.y * weight;
-            const float* x = p.partial + at * kDim + lane * kCols;      // (zeros where this part saw nothing)
+    for (int e = 0; e < kCols; ++e) sum[e] = 0.0f;
+#pragma unroll 8
+    for (int i = first; i <= last; ++i) {                   // (slot 1: the CTA that has tile 0; slot 0: the ones after it)
+        const int64_t at = ((int64_t)i * 2 + (i == first)) * rows + r;
+        const float2 w = *reinterpret_cast<const float2*>(ml + at * 2);
+        const float* x = p.partial + at * kDim + lane * kCols;      // (zeros where this part saw nothing)
+        float v[kCols];
 #pragma unroll
-            for (int e = 0; e < kCols; ++e) sum[e] += x[e] * weight;
-        }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        T* to = static_cast<T*>(p.o) + (((int64_t)b * p.drafts + draft) * (p.kv_heads * p.group) + head * p.group + (row - draft * p.group)) * kDim + lane * kCols;
+        for (int e = 0; e < kCols; e += 2) *reinterpret_cast<float2*>(v + e) = *reinterpret_cast<const float2*>(x + e);
+        const float weight = attn_exp2(w.x - ref);
+        l += w.y * weight;
 #pragma unroll
-        for (int e = 0; e < kCols; ++e) to[e] = Scalar<T>::from_float(sum[e] * inv);
+        for (int e = 0; e < kCols; ++e) sum[e] += v[e] * weight;
     }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* to = static_cast<T*>(p.o) + (((int64_t)b * p.drafts + draft) * (p.kv_heads * p.group) + head * p.group + (row - draft * p.group)) * kDim + lane * kCols;
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) to[e] = Scalar<T>::from_float(sum[e] * inv);
 }
 
 // Map of a side of the cache as rows of head_dim elements, one page (at most a tile of it) per box.
@@ -673,7 +692,7 @@ int launch_cached(const CachedParams& p, const CUtensorMap& map_k, const CUtenso
     constexpr int smem = CachedShape<kE4m3, kDim>::kSmem;
     if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return BSA_ERR_LAUNCH;
     kernel<<<p.ctas, (kConsumers + 1) * 32, smem, stream>>>(p, map_k, map_v);
-    cached_join_kernel<T, kDim><<<p.batch * p.kv_heads * p.row_tiles, 128, 0, stream>>>(p, 16 * kGroups);
+    cached_join_kernel<T, kDim><<<p.batch * p.kv_heads * p.row_tiles * 4 * kGroups, 128, 0, stream>>>(p, 16 * kGroups);
     return launch_status();
 }
 template <typename T, bool kE4m3, int kDim>
@@ -728,7 +747,7 @@ extern "C" int bsa_cached_attention(int dtype, int store, const void* q, int64_t
     const int64_t group = q_heads / kv_heads;
     const int groups = row_groups(drafts * group);
     const int64_t row_tiles = (drafts * group + 16 * groups - 1) / (16 * groups);
-    if (row_tiles * kv_heads > (int64_t)INT32_MAX / batch || q_heads > 65535) return BSA_ERR_TOO_LARGE;
+    if (row_tiles * kv_heads > (int64_t)INT32_MAX / batch / (4 * groups) || q_heads > 65535) return BSA_ERR_TOO_LARGE;
     p.q = q; p.o = o;
     p.q_batch = q_batch_stride; p.q_draft = q_draft_stride; p.q_head = q_head_stride;
     p.scales[0] = key_scales; p.scales[1] = value_scales;
