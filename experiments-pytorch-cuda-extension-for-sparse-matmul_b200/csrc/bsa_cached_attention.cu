@@ -19,7 +19,7 @@
 //
 // e4m3 caches.  Codes are exact in fp16, so the products run in fp16 on the codes themselves and the scales go where they
 // are cheap: the key's into the score, and the value's into the weight: with y_ij = log2(e) scale q_i k_j + log2 sv_j the
-// weights are P_ij = 2^(y_ij - m_i), m_i the running maximum of y (so P <= 1 whatever the scales are), O += P code,
+// weights are P_ij = 2^(y_ij - m_i), m_i the running maximum of y (so P <= 2^8 whatever the scales are), O += P code,
 // l += P / sv_j, o = O / l.  bf16 queries are brought to fp16 by a power of two per row (exact but for values below
 // 2^-14 of the row's largest).  The 8-bit elements are paired by ldmatrix as 16-bit units, which permutes the
 // contraction axis of Q K^T (the query is loaded in the same order) and the columns of O (undone at the store).
@@ -54,6 +54,7 @@ struct CachedParams {
     int batch, drafts, group, kv_heads, row_tiles, table_width, pages, page_shift;
     float scale_log2;                           // scale * log2 e
     float* partial;                             // [ctas][2][rows][head_dim], then [ctas][2][rows][2] of (m, l)
+    int2* parts;                                // [batch][kv_heads * row_tiles]: first and last CTA of each
     int ctas;
     uint32_t* status;
 };
@@ -78,22 +79,18 @@ __device__ __forceinline__ int cached_tiles(const CachedParams& p, int b) {
     return max(1, (cached_length(p, b) + kTileKeys - 1) / kTileKeys);
 }
 
-// Cost of one head and row tile of sequences 0 .. end - 1 (all of them before `part`, in `before`), by one warp.
-__device__ __forceinline__ int64_t total_cost(const CachedParams& p, int part, int64_t& before, int lane) {
-    int64_t sum = 0, some = 0;
+// Units of one head and row tile of the whole batch, by one warp.
+__device__ __forceinline__ int64_t total_cost(const CachedParams& p, int lane) {
+    int64_t sum = 0;
 #pragma unroll 4
-    for (int b = lane; b < p.batch; b += 32) {
-        const int cost = cached_tiles(p, b) + kBegin;
-        sum += cost;
-        if (b < part) some += cost;
-    }
+    for (int b = lane; b < p.batch; b += 32) sum += cached_tiles(p, b) + kBegin;
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, s);
-        some += __shfl_xor_sync(0xffffffffu, some, s);
-    }
-    before = some;
+    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
     return sum;
+}
+// a / b; the units fit 32 bits unless a batch holds more keys than the device's memory
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
 // A (sequence, head, row tile) takes kBegin + tiles units of the list, its tiles last.  Finds where this CTA's share
@@ -101,9 +98,8 @@ __device__ __forceinline__ int64_t total_cost(const CachedParams& p, int part, i
 __device__ __forceinline__ Share find_share(const CachedParams& p, int cta, int lane) {
     Share s;
     const int hms = p.kv_heads * p.row_tiles;
-    int64_t none;
-    const int64_t units = total_cost(p, 0, none, lane) * hms;
-    s.per = (units + p.ctas - 1) / p.ctas;
+    const int64_t units = total_cost(p, lane) * hms;
+    s.per = quotient(units + p.ctas - 1, p.ctas);
     s.first = min((int64_t)cta * s.per, units);
     s.end = min(s.first + s.per, units);
     s.b = s.hm = s.tile = 0;
@@ -124,7 +120,7 @@ __device__ __forceinline__ Share find_share(const CachedParams& p, int cta, int 
             const int64_t start = before + __shfl_sync(0xffffffffu, upto, l) - cost;
             const int64_t off = s.first - start * hms;
             s.b = b0 + l;
-            s.hm = (int)(off / cost);
+            s.hm = (int)quotient(off, cost);
             const int within = (int)(off - (int64_t)s.hm * cost);
             s.tile = max(within - kBegin, 0);
             s.first += max(kBegin - within, 0);             // the unit of that tile
@@ -133,6 +129,11 @@ __device__ __forceinline__ Share find_share(const CachedParams& p, int cta, int 
         before += __shfl_sync(0xffffffffu, upto, 31);
     }
     return s;
+}
+
+// How many CTAs after this one hold tiles of an item whose last unit is `last` (from the share's nominal end on).
+__device__ __forceinline__ int later_parts(int64_t last, const Share& s) {
+    return last < s.end ? 0 : 1 + (int)((uint32_t)min(last - s.end, (int64_t)UINT32_MAX) / (uint32_t)s.per);
 }
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
@@ -219,7 +220,13 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
     uint32_t phase = 0;
 
     if (warp == kConsumers) {                               // ---- producer
+        // One lane per copy of a tile, so that all leave with one instruction: pages (at most 4) x sides x panels of the
+        // keys and values in lanes 0-15, pages x sides of the scales in lanes 16-23.  (Issued one after another by the
+        // pages' lanes they took longer than the tile's arithmetic.)
         const int page = 1 << p.page_shift, piece = min(page, kTileKeys), pieces = kTileKeys / piece;
+        const int my_piece = lane & 3, my_side = (lane >> 2) & 1, my_panel = (lane >> 3) & 1;
+        const bool my_scale = kE4m3 && lane >= 16 && lane < 24, my_tile = lane < 8 * S::kPanels;
+        const CUtensorMap* my_map = my_side == 0 ? &map_k : &map_v;
         bool dead = false;
         int64_t u = share.first;
         int length = 0, tiles = 0, id = 0;
@@ -229,15 +236,15 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             if (lane == 0 && p.lengths[b] != length) atomicExch(p.status, (uint32_t)BSA_ERR_BAD_SHAPE);
         };
         auto look = [&]() {                                 // this lane's page of the tile
-            const int key = tile * kTileKeys + lane * piece;
+            const int key = tile * kTileKeys + my_piece * piece;
             id = 0;
-            if (lane < pieces && key < length) id = p.table[(int64_t)b * p.table_width + (key >> p.page_shift)];
+            if (my_piece < pieces && key < length) id = p.table[(int64_t)b * p.table_width + (key >> p.page_shift)];
         };
         if (u < share.end) { enter(); look(); }
         while (u < share.end) {
             const int head = hm / p.row_tiles;
-            const int key = tile * kTileKeys + lane * piece;
-            bool ok = lane < pieces && key < length;
+            const int key = tile * kTileKeys + my_piece * piece;
+            bool ok = my_piece < pieces && key < length;
             if (ok && (uint32_t)id >= (uint32_t)p.pages) {  // not a page of this cache: its keys are left out, and reported
                 atomicExch(p.status, (uint32_t)BSA_ERR_BAD_SHAPE);
                 ok = false;
@@ -255,7 +262,7 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
                 }
             }
             if (u < share.end) look();
-            const uint32_t loaded = __ballot_sync(0xffffffffu, ok);
+            const uint32_t loaded = __ballot_sync(0xffffffffu, ok) & 15u;
             dead = !mbar_wait(&bars->empty[stage], phase ^ 1, &bars->abort_flag, p.status);
             if (dead) break;
             if (lane == 0) {
@@ -263,20 +270,14 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
                 mbar_expect_tx(&bars->full[stage], (uint32_t)(__popc(loaded) * piece * (2 * S::kRowBytes + (kE4m3 ? 8 : 0))));
             }
             __syncwarp();
-            if (ok) {
-                uint8_t* base = smem + stage * S::kStageBytes;
-#pragma unroll
-                for (int side = 0; side < 2; ++side) {
-                    const CUtensorMap* map = side == 0 ? &map_k : &map_v;
-#pragma unroll
-                    for (int panel = 0; panel < S::kPanels; ++panel)
-                        tma_load_3d(base + side * S::kSideBytes + panel * (kTileKeys * S::kPanelBytes) + lane * piece * S::kPanelBytes,
-                                    map, &bars->full[stage], panel * (S::kPanelBytes / (kE4m3 ? 1 : 2)), row, 0);
-                    if (kE4m3)
-                        bulk_load_1d(scale_smem + stage * S::kScaleBytes + side * (kTileKeys * 4) + lane * piece * 4,
-                                     p.scales[side] + row, (uint32_t)(piece * 4), &bars->full[stage]);
-                }
-            }
+            if (ok && my_tile)
+                tma_load_3d(smem + stage * S::kStageBytes + my_side * S::kSideBytes + my_panel * (kTileKeys * S::kPanelBytes) +
+                            my_piece * piece * S::kPanelBytes, my_map, &bars->full[stage],
+                            my_panel * (S::kPanelBytes / (kE4m3 ? 1 : 2)), row, 0);
+            if (ok && my_scale)
+                bulk_load_1d(scale_smem + stage * S::kScaleBytes + my_side * (kTileKeys * 4) + my_piece * piece * 4,
+                             p.scales[my_side] + row, (uint32_t)(piece * 4), &bars->full[stage]);
+            __syncwarp();
             if (++stage == S::kStages) { stage = 0; phase ^= 1; }
         }
         if (dead) let_copies_land();
@@ -463,23 +464,19 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
                     }
                 }
             }
-            // running maximum
+            // The running maximum is raised only where a score exceeds it by more than 8 (units of log2): P stays below
+            // 2^8, and O and l carry the same factor whatever it is.
             float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int n = 0; n < kNT; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
             float ref[2];
-            bool raise = false;
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                raise |= top[r] > m[r];
-            }
-            if (__any_sync(0xffffffffu, raise)) {
+            if (__any_sync(0xffffffffu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f)) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
                     const float higher = fmaxf(m[r], top[r]);
                     const float fall = higher == -INFINITY ? 1.0f : attn_exp2(m[r] - higher);
                     m[r] = higher;
@@ -572,6 +569,8 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             }
             asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
         }
+        if (from_start && threadIdx.x == 0)
+            p.parts[(int64_t)b * hms + hm] = make_int2((int)blockIdx.x, (int)blockIdx.x + later_parts(u + tiles - 1, share));
         if (part == 0) {
             const int slot = from_start ? 1 : 0;
             const int64_t part_row = ((int64_t)blockIdx.x * 2 + slot) * kRows + rg * 16 + g;
@@ -621,6 +620,8 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             if (++hm == hms) { hm = 0; ++b; }
         }
     }
+    // the join may be scheduled once every CTA is here (it waits for their memory itself)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 // Joins what several CTAs left of one (sequence, key head, row tile): one warp per row, kDim / 32 columns per lane.
@@ -633,11 +634,9 @@ cached_join_kernel(const CachedParams p, int rows) {
     const int b = item / hms, hm = item - b * hms;
     const int head = hm / p.row_tiles, row = (hm - head * p.row_tiles) * rows + r, draft = row / p.group;
     if (draft >= p.drafts) return;
-    int64_t before;
-    const int64_t per = (total_cost(p, b, before, lane) * hms + p.ctas - 1) / p.ctas;
-    const int tiles = cached_tiles(p, b);
-    const int64_t start = before * hms + (int64_t)hm * (tiles + kBegin) + kBegin;       // the unit of tile 0
-    const int first = (int)(start / per), last = (int)((start + tiles - 1) / per);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int2 parts = p.parts[item];
+    const int first = parts.x, last = parts.y;
     if (first == last) return;                              // one CTA had all of it and wrote the output
     const float* ml = p.partial + (int64_t)p.ctas * 2 * rows * kDim;
     constexpr int kCols = kDim / 32;
@@ -692,7 +691,17 @@ int launch_cached(const CachedParams& p, const CUtensorMap& map_k, const CUtenso
     constexpr int smem = CachedShape<kE4m3, kDim>::kSmem;
     if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return BSA_ERR_LAUNCH;
     kernel<<<p.ctas, (kConsumers + 1) * 32, smem, stream>>>(p, map_k, map_v);
-    cached_join_kernel<T, kDim><<<p.batch * p.kv_heads * p.row_tiles * 4 * kGroups, 128, 0, stream>>>(p, 16 * kGroups);
+    // the join's CTAs may start while the last ones above end; they wait for all of them before they read
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((unsigned)(p.batch * p.kv_heads * p.row_tiles * 4 * kGroups));
+    config.blockDim = dim3(128);
+    config.stream = stream;
+    cudaLaunchAttribute overlap{};
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &overlap;
+    config.numAttrs = 1;
+    if (cudaLaunchKernelEx(&config, cached_join_kernel<T, kDim>, p, 16 * kGroups) != cudaSuccess) { cudaGetLastError(); return BSA_ERR_LAUNCH; }
     return launch_status();
 }
 template <typename T, bool kE4m3, int kDim>
@@ -714,10 +723,11 @@ int launch_cached_typed(int store, int64_t dim, int groups, const CachedParams& 
 }  // namespace
 }  // namespace bsa
 
-extern "C" size_t bsa_cached_attention_scratch(int64_t drafts, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
-    if (drafts <= 0 || kv_heads <= 0 || q_heads < kv_heads || head_dim <= 0) return 0;
-    const int sms = bsa::sm_count();
-    return (size_t)std::max(sms, 1) * 2 * 2 * 16 * bsa::row_groups(drafts * (q_heads / kv_heads)) * (size_t)(head_dim + 2) * 4;
+extern "C" size_t bsa_cached_attention_scratch(int64_t batch, int64_t drafts, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
+    if (batch <= 0 || drafts <= 0 || kv_heads <= 0 || q_heads < kv_heads || head_dim <= 0) return 0;
+    const int64_t rows = drafts * (q_heads / kv_heads), tile = 16 * bsa::row_groups(rows);
+    const size_t parts = (size_t)batch * kv_heads * ((rows + tile - 1) / tile) * sizeof(int2);
+    return parts + (size_t)std::max(bsa::sm_count(), 1) * 2 * 2 * tile * (size_t)(head_dim + 2) * 4;
 }
 
 extern "C" int bsa_cached_attention(int dtype, int store, const void* q, int64_t q_batch_stride, int64_t q_draft_stride,
@@ -763,7 +773,8 @@ extern "C" int bsa_cached_attention(int dtype, int store, const void* q, int64_t
     p.ctas = 2 * sm_count();
     p.status = static_cast<uint32_t*>(workspace);
     if (p.ctas <= 0) return BSA_ERR_LAUNCH;
-    if (scratch_bytes < bsa_cached_attention_scratch(drafts, q_heads, kv_heads, head_dim)) return BSA_ERR_WORKSPACE;
+    p.parts = reinterpret_cast<int2*>(p.partial + (int64_t)p.ctas * 2 * 16 * groups * (head_dim + 2));
+    if (scratch_bytes < bsa_cached_attention_scratch(batch, drafts, q_heads, kv_heads, head_dim)) return BSA_ERR_WORKSPACE;
     // the driver's encoder needs the device's context bound to this thread
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) { cudaGetLastError(); return BSA_ERR_LAUNCH; }
