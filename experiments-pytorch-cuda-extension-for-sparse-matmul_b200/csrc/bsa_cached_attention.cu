@@ -25,8 +25,6 @@
 // contraction axis of Q K^T (the query is loaded in the same order) and the columns of O (undone at the store).
 //
 // P is rounded to the products' 16-bit type (relative 2^-9 in bf16, 2^-12 in fp16), l, m and O are fp32.
-#include <cuda_fp8.h>
-
 #include <algorithm>
 #include <type_traits>
 
@@ -37,7 +35,7 @@ namespace {
 
 constexpr int kTileKeys = 64;
 constexpr int kConsumers = 4;                   // warps
-constexpr int kBegin = 3;                       // what beginning and ending a (sequence, head) costs a CTA, in tiles
+constexpr int kBegin = 6;                       // what beginning and ending a (sequence, head) costs a CTA, in tiles
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct CachedParams {
@@ -155,13 +153,13 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// two e4m3 codes (low 16 bits) as two fp16 values
-__device__ __forceinline__ uint32_t halves2(uint32_t codes) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3);
-    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+// Four e4m3 codes as fp16 values: codes 0, 1 and codes 2, 3.
+__device__ __forceinline__ void halves4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(codes));
 }
 
-template <bool kE4m3, int kDim>
+template <bool kE4m3, int kDim, int kGroups>
 struct CachedShape {
     static constexpr int kRowBytes = kDim * (kE4m3 ? 1 : 2);
     static constexpr int kPanelBytes = kRowBytes < 128 ? kRowBytes : 128;       // width of a TMA box
@@ -169,37 +167,46 @@ struct CachedShape {
     static constexpr int kSideBytes = kTileKeys * kRowBytes;
     static constexpr int kScaleBytes = kE4m3 ? 2 * kTileKeys * 4 : 0;
     static constexpr int kStageBytes = 2 * kSideBytes;
-    // two CTAs per SM: 113 KB each, of which the merge buffers take up to 17
     static constexpr int kStages = kStageBytes >= 32768 ? 3 : (kStageBytes >= 16384 ? 5 : 8);
-    static constexpr int kMergeBytes = 2 * 16 * kDim * 4 + 2 * 32 * 4 * 4;
-    static constexpr int kSmem = kStages * (kStageBytes + kScaleBytes) + kMergeBytes + (int)sizeof(CachedBarriers<kStages>);
+    // columns of O that the warps of a row group join at a time (the 8-bit layout stores pairs of 8-column tiles)
+    static constexpr int kJoin = kE4m3 ? 64 : 32;
+    static constexpr int kJoinFloats = kGroups == 4 ? 0 : kConsumers * 16 * (kJoin + 2);
+    static constexpr int kRows = 16 * kGroups;
+    static constexpr int kQueryBytes = kRows * (kDim * 2 + 4);                  // fragments, and a factor per row
+    static constexpr int kSmem = kStages * (kStageBytes + kScaleBytes) + kQueryBytes + kJoinFloats * 4 + (int)sizeof(CachedBarriers<kStages>);
+    static_assert(2 * (kSmem + 1024) <= 233472, "two CTAs per SM");
 };
-// Byte offset of 16-byte chunk `chunk` of key `key` inside a side of a stage, as the TMA swizzle leaves it.
-template <bool kE4m3, int kDim>
-__device__ __forceinline__ uint32_t chunk_offset(int key, int chunk) {
-    using S = CachedShape<kE4m3, kDim>;
-    if (S::kPanelBytes == 128)
-        return (uint32_t)((chunk >> 3) * (kTileKeys * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
-    return (uint32_t)(key * 64 + ((chunk ^ ((key >> 1) & 3)) << 4));
+
+// Where the TMA swizzle leaves 16-byte chunk `chunk` of row `row` (of 8 or 16 rows that start on a multiple of 8).
+template <int kPanelBytes>
+__device__ __forceinline__ uint32_t chunk_offset(int row, int chunk) {
+    if (kPanelBytes == 128)
+        return (uint32_t)((chunk >> 3) * (kTileKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+    return (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
 }
 
 // T: type of q and o; kGroups: groups of 16 rows (1, 2 or 4).
 template <typename T, bool kE4m3, int kDim, int kGroups>
 __global__ void __launch_bounds__((kConsumers + 1) * 32, 2)
 cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
-    using S = CachedShape<kE4m3, kDim>;
+    using S = CachedShape<kE4m3, kDim, kGroups>;
     using Bars = CachedBarriers<S::kStages>;
     constexpr bool kTBf16 = std::is_same_v<T, __nv_bfloat16>;
     constexpr bool kBf16 = !kE4m3 && kTBf16;                // type of the products
     constexpr int kRows = 16 * kGroups;
     constexpr int kSplit = kConsumers / kGroups;            // warps that share a row group
-    constexpr int kWarpKeys = kTileKeys / kSplit;           // keys of a tile per warp
+    // With one row group the warps work as two pairs on alternate tiles, 32 keys each: 16 keys per warp and tile leave
+    // too few independent instructions between the tile's barriers.
+    constexpr int kStreams = kSplit == 4 ? 2 : 1;
+    constexpr int kWarpKeys = kTileKeys * kStreams / kSplit;            // keys of a tile per warp
     constexpr int kStepKeys = kWarpKeys < 32 ? kWarpKeys : 32;          // keys of a step of the warp (registers)
     constexpr int kNT = kStepKeys / 8;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* scale_smem = smem + S::kStages * S::kStageBytes;
-    float* merge = reinterpret_cast<float*>(scale_smem + S::kStages * S::kScaleBytes);
-    Bars* bars = reinterpret_cast<Bars*>(reinterpret_cast<uint8_t*>(merge) + S::kMergeBytes);
+    uint32_t* q_smem = reinterpret_cast<uint32_t*>(scale_smem + S::kStages * S::kScaleBytes);     // [row group][k step][lane][4]
+    float* q_factor = reinterpret_cast<float*>(q_smem + kRows * kDim / 2);
+    float* merge = q_factor + kRows;
+    Bars* bars = reinterpret_cast<Bars*>(merge + S::kJoinFloats);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0) {
         const Share mine = find_share(p, (int)blockIdx.x, lane);
@@ -208,7 +215,7 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
         bars->abort_flag = 0;
         for (int i = 0; i < S::kStages; ++i) {
             mbar_init(&bars->full[i], 1);
-            mbar_init(&bars->empty[i], kConsumers);
+            mbar_init(&bars->empty[i], kConsumers / kStreams);
         }
         fence_async_shared();
     }
@@ -285,89 +292,90 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
     }
 
     // ---- consumers
-    const int rg = warp / kSplit, part = warp % kSplit;     // row group; which keys of a tile
+    const int rg = warp / kSplit, part = warp % kSplit;     // row group; number among its warps
+    const int stream = part % kStreams, first_key = part / kStreams * kWarpKeys;        // which tiles, which keys of them
+    uint32_t turn = 0;                                      // tiles so far
     const int g = lane >> 2, c = lane & 3;
+    // addresses of this lane's ldmatrix rows inside 8 keys (K) and 16 keys (V)
+    uint32_t k_lane[S::kRowBytes / 64];
+#pragma unroll
+    for (int x = 0; x < S::kRowBytes / 64; ++x) k_lane[x] = chunk_offset<S::kPanelBytes>(lane & 7, 4 * x + (lane >> 3));
+    const uint32_t v_lane = chunk_offset<S::kPanelBytes>(lane & 15, lane >> 4);
     bool dead = false;
     int64_t u = share.first;
+    // The queries of the next (sequence, head, row tile) are fetched before the one at hand is joined and stored, so that
+    // they travel meanwhile; they go to shared memory in the order of the fragments.
+    constexpr int kChunks = kDim / 8, kLoads = (kRows * kChunks + kConsumers * 32 - 1) / (kConsumers * 32);
     int at_b = -1, length = 0, tiles = 0, count = 0;
-    while (u < share.end) {
+    uint64_t sees[2];                                       // of this thread's two rows: the drafts that it sees,
+    int row_block[2];                                       // its block row in the pattern,
+    bool row_on[2];                                         // and whether it is one of the sequence's drafts
+    uint4 fetched[kLoads];
+    auto fetch = [&]() {
         if (b != at_b) {
             at_b = b;
             length = cached_length(p, b);
-            tiles = max(1, (length + kTileKeys - 1) / kTileKeys);
             count = p.counts ? min(max(p.counts[b], 0), p.drafts) : p.drafts;
+            tiles = max(1, (length + kTileKeys - 1) / kTileKeys);
         }
-        const int prefix = length - count;                  // negative where a sequence has fewer tokens than drafts
         const int head = hm / p.row_tiles, row_tile = hm - head * p.row_tiles;
-        const int todo = (int)min((int64_t)(tiles - tile), share.end - u);
-        const bool whole = tile == 0 && todo == tiles;
-        const bool from_start = tile == 0;
-
-        // this thread's two rows
-        uint64_t sees[2];
-        int row_block[2];
-        bool live[2];
-        int64_t q_at[2], o_at[2];
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int chunk = (int)threadIdx.x + i * kConsumers * 32;
+            const int row = row_tile * kRows + chunk / kChunks, draft = row / p.group, h = head * p.group + row - draft * p.group;
+            fetched[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (chunk < kRows * kChunks && draft < count)   // (drafts behind the sequence's own are zeros, and masked)
+                fetched[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_batch + draft * p.q_draft + h * p.q_head + chunk % kChunks * 8);
+        }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const int row = row_tile * kRows + rg * 16 + g + 8 * r;
-            const int draft = row / p.group, of_group = row - draft * p.group;
-            live[r] = draft < p.drafts;
-            const int h = head * p.group + of_group;
-            q_at[r] = b * p.q_batch + draft * p.q_draft + h * p.q_head;
-            o_at[r] = (((int64_t)b * p.drafts + draft) * (p.kv_heads * p.group) + h) * kDim;
+            const int draft = (row_tile * kRows + rg * 16 + g + 8 * r) / p.group;
+            row_on[r] = draft < count;
             sees[r] = 0;
             row_block[r] = -1;
-            if (live[r] && draft < count) {
+            if (row_on[r]) {
                 sees[r] = p.tree ? (uint64_t)p.tree[(int64_t)b * p.drafts + draft] : ~0ull >> (63 - draft);
                 // a draft stands behind the prefix and its ancestors: its depth is the number of those
-                if (p.pattern) row_block[r] = (max(prefix, 0) + max(__popcll(sees[r]) - 1, 0)) >> p.pattern_shift;
+                if (p.pattern) row_block[r] = (max(length - count, 0) + max(__popcll(sees[r]) - 1, 0)) >> p.pattern_shift;
             }
         }
-        const bool row_on[2] = {live[0] && (row_tile * kRows + rg * 16 + g) / p.group < count,
-                                live[1] && (row_tile * kRows + rg * 16 + g + 8) / p.group < count};
-
-        // query fragments
-        uint32_t qf[kDim / 16][4];
-        float row_scale[2] = {p.scale_log2, p.scale_log2};
-        if (!kE4m3) {
+    };
+    auto put = [&]() {
 #pragma unroll
-            for (int s = 0; s < kDim / 16; ++s)
+        for (int i = 0; i < kLoads; ++i) {
+            const int chunk = (int)threadIdx.x + i * kConsumers * 32, row = chunk / kChunks, at = chunk % kChunks;
+            uint32_t w[4] = {fetched[i].x, fetched[i].y, fetched[i].z, fetched[i].w};
+            if (kE4m3 && kTBf16) {                          // bf16 queries to fp16 by a power of two per row
+                uint32_t top = 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = e & 1;
-                    qf[s][e] = row_on[r] ? *reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + q_at[r] + 16 * s + 2 * c + 8 * (e >> 1)) : 0u;
-                }
-        } else {
-            uint2 raw[kDim / 16][2];
-            uint32_t top[2] = {0, 0};
+                for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fff0000u, w[e] << 16 & 0x7fff0000u));
 #pragma unroll
-            for (int s = 0; s < kDim / 16; ++s)
+                for (int d = kChunks / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const int e = min(max((int)(top >> 23), 1), 253);                // biased exponent of the row's largest
+                const float down = __uint_as_float((uint32_t)(254 - e) << 23);    // 2^-(e - 127)
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    raw[s][r] = row_on[r] ? *reinterpret_cast<const uint2*>(static_cast<const T*>(p.q) + q_at[r] + 16 * s + 4 * c) : make_uint2(0u, 0u);
-                    const T* x = reinterpret_cast<const T*>(&raw[s][r]);
+                for (int x = 0; x < 4; ++x)
+                    w[x] = pack2<false>(__uint_as_float(w[x] << 16) * down, __uint_as_float(w[x] & 0xffff0000u) * down);
+                if (at == 0 && row < kRows) q_factor[row] = p.scale_log2 * __uint_as_float((uint32_t)e << 23);
+            }
+            if (row < kRows) {
+                // k step at / 2; the fragment of lane 4 (row % 8) + c holds the words (row, row + 8) x (first, second pair)
+                uint32_t* to = q_smem + (((row / 16) * (kDim / 16) + at / 2) * 32 + (row & 7) * 4) * 4 + ((row >> 3) & 1);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top[r] = max(top[r], __float_as_uint(Scalar<T>::to_float(x[e])) & 0x7fffffffu);
-                }
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                float down = 1.0f;
-                if (kTBf16) {
-                    top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                    top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                    const int e = min(max((int)(top[r] >> 23), 1), 253);         // biased exponent of the row's largest
-                    down = __uint_as_float((uint32_t)(254 - e) << 23);            // 2^-(e - 127)
-                    row_scale[r] = p.scale_log2 * __uint_as_float((uint32_t)e << 23);
-                }
-#pragma unroll
-                for (int s = 0; s < kDim / 16; ++s) {
-                    const T* x = reinterpret_cast<const T*>(&raw[s][r]);
-                    qf[s][r] = pack2<false>(Scalar<T>::to_float(x[0]) * down, Scalar<T>::to_float(x[1]) * down);
-                    qf[s][2 + r] = pack2<false>(Scalar<T>::to_float(x[2]) * down, Scalar<T>::to_float(x[3]) * down);
-                }
+                for (int x = 0; x < 4; ++x)
+                    to[kE4m3 ? (2 * (at & 1) + x / 2) * 4 + 2 * (x & 1) : x * 4 + 2 * (at & 1)] = w[x];
             }
         }
+        asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
+    };
+    if (u < share.end) fetch();
+    while (u < share.end) {
+        put();
+        const int prefix = length - count;                  // negative where a sequence has fewer tokens than drafts
+        const int todo = (int)min((int64_t)(tiles - tile), share.end - u);
+        const bool from_start = tile == 0, whole = from_start && todo == tiles;
+        const uint4* q_frag = reinterpret_cast<const uint4*>(q_smem) + rg * (kDim / 16) * 32 + lane;
+        const float row_scale[2] = {kE4m3 && kTBf16 ? q_factor[rg * 16 + g] : p.scale_log2, kE4m3 && kTBf16 ? q_factor[rg * 16 + g + 8] : p.scale_log2};
 
         float out[kDim / 8][4];
 #pragma unroll
@@ -376,12 +384,16 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             for (int e = 0; e < 4; ++e) out[i][e] = 0.0f;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
-        for (int i = 0; i < todo; ++i, ++tile) {
+        for (int i = 0; i < todo; ++i, ++tile, ++turn) {
+            if (kStreams == 2 && (int)(turn & 1) != stream) {
+                if (++stage == S::kStages) { stage = 0; phase ^= 1; }
+                continue;
+            }
             if (!dead) dead = !mbar_wait(&bars->full[stage], phase, &bars->abort_flag, p.status);
             const uint32_t k_base = smem_u32(smem) + stage * S::kStageBytes, v_base = k_base + S::kSideBytes;
             const uint32_t loaded = bars->ok[stage];
 #pragma unroll 1
-            for (int base = part * kWarpKeys; base < (part + 1) * kWarpKeys; base += kStepKeys) {
+            for (int base = first_key; base < first_key + kWarpKeys; base += kStepKeys) {
             const int key0 = tile * kTileKeys + base;
             float s[kNT][4];
 #pragma unroll
@@ -389,24 +401,30 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
             // Q K^T
+            const uint32_t rows8 = k_base + (uint32_t)(base * S::kPanelBytes);
 #pragma unroll
-            for (int n = 0; n < kNT; ++n) {
-                const int key = base + n * 8 + (lane & 7);
-                if (!kE4m3) {
+            for (int x = 0; x < S::kRowBytes / 64; ++x) {
+                constexpr int kSteps = kE4m3 ? 4 : 2;       // k steps of 64 bytes of a key
+                uint32_t qf[kSteps][4];
 #pragma unroll
-                    for (int x = 0; x < kDim / 32; ++x) {
-                        uint32_t kf[4];
-                        ldsm_x4(k_base + chunk_offset<kE4m3, kDim>(key, 4 * x + (lane >> 3)), kf);
-                        mma_16816<kBf16>(s[n], qf[2 * x], kf[0], kf[1]);
-                        mma_16816<kBf16>(s[n], qf[2 * x + 1], kf[2], kf[3]);
-                    }
-                } else {
+                for (int e = 0; e < kSteps; ++e) {
+                    const uint4 w = q_frag[(kSteps * x + e) * 32];
+                    qf[e][0] = w.x; qf[e][1] = w.y; qf[e][2] = w.z; qf[e][3] = w.w;
+                }
 #pragma unroll
-                    for (int x = 0; x < kDim / 64; ++x) {
-                        uint32_t kf[4];
-                        ldsm_x4(k_base + chunk_offset<kE4m3, kDim>(key, 4 * x + (lane >> 3)), kf);
+                for (int n = 0; n < kNT; ++n) {
+                    uint32_t kf[4];
+                    ldsm_x4(rows8 + (uint32_t)(n * 8 * S::kPanelBytes) + k_lane[x], kf);
+                    if (!kE4m3) {
+                        mma_16816<kBf16>(s[n], qf[0], kf[0], kf[1]);
+                        mma_16816<kBf16>(s[n], qf[kSteps / 2], kf[2], kf[3]);
+                    } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) mma_16816<false>(s[n], qf[4 * x + e], halves2(kf[e]), halves2(kf[e] >> 16));
+                        for (int e = 0; e < kSteps; ++e) {
+                            uint32_t b0, b1;
+                            halves4(kf[e], b0, b1);
+                            mma_16816<false>(s[n], qf[e], b0, b1);
+                        }
                     }
                 }
             }
@@ -503,11 +521,12 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
                 const uint32_t pf[4] = {pack2<kBf16>(s[2 * ks][0], s[2 * ks][1]), pack2<kBf16>(s[2 * ks][2], s[2 * ks][3]),
                                         pack2<kBf16>(s[2 * ks + 1][0], s[2 * ks + 1][1]), pack2<kBf16>(s[2 * ks + 1][2], s[2 * ks + 1][3])};
                 // lanes 0-7: keys 0-7 of the step, chunk a; 8-15: keys 8-15, chunk a; 16-31: the same of chunk a + 1
-                const int key = base + ks * 16 + (lane & 15);
+                const uint32_t rows16 = v_base + (uint32_t)((base + ks * 16) * S::kPanelBytes) + v_lane;
 #pragma unroll
                 for (int a = 0; a < S::kRowBytes / 16; a += 2) {
                     uint32_t vf[4];
-                    ldsm_x4_trans(v_base + chunk_offset<kE4m3, kDim>(key, a + (lane >> 4)), vf);
+                    // (a is even, so the chunk's number goes into the swizzled address as an exclusive or)
+                    ldsm_x4_trans((rows16 ^ (uint32_t)((a & 7) << 4)) + (uint32_t)((a >> 3) * (kTileKeys * 128)), vf);
                     if (masked) {                           // what is not there may be anything, a NaN too
                         vf[0] &= keep[2 * ks]; vf[1] &= keep[2 * ks + 1];
                         vf[2] &= keep[2 * ks]; vf[3] &= keep[2 * ks + 1];
@@ -519,8 +538,11 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {       // bytes (0, 2): even columns of the chunk, (1, 3): odd ones
                             const uint32_t w0 = __byte_perm(vf[2 * x], 0, 0x3120), w1 = __byte_perm(vf[2 * x + 1], 0, 0x3120);
-                            mma_16816<false>(out[2 * (a + x)], pf, halves2(w0), halves2(w1));
-                            mma_16816<false>(out[2 * (a + x) + 1], pf, halves2(w0 >> 16), halves2(w1 >> 16));
+                            uint32_t even0, odd0, even1, odd1;
+                            halves4(w0, even0, odd0);
+                            halves4(w1, even1, odd1);
+                            mma_16816<false>(out[2 * (a + x)], pf, even0, even1);
+                            mma_16816<false>(out[2 * (a + x) + 1], pf, odd0, odd1);
                         }
                     }
                 }
@@ -536,88 +558,105 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
         }
-        // the warps that share a row group: the upper half hands its (O, m, l) to the lower until one is left
-#pragma unroll
-        for (int half = kSplit / 2; half > 0; half >>= 1) {
-            const int buffer = kGroups == 1 ? part % half : rg % 2;
-            float* mo = merge + buffer * (16 * kDim);
-            float* ml = merge + 2 * 16 * kDim + buffer * 128;
-            if (part >= half && part < 2 * half) {
-#pragma unroll
-                for (int d = 0; d < kDim / 8; ++d)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) mo[(d * 4 + e) * 32 + lane] = out[d][e];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) { ml[r * 32 + lane] = m[r]; ml[64 + r * 32 + lane] = l[r]; }
-            }
-            asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
-            if (part < half) {
-                float mine[2], theirs[2];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float om = ml[r * 32 + lane], higher = fmaxf(m[r], om);
-                    const float ref = higher == -INFINITY ? 0.0f : higher;
-                    mine[r] = attn_exp2(m[r] - ref);
-                    theirs[r] = attn_exp2(om - ref);
-                    l[r] = l[r] * mine[r] + ml[64 + r * 32 + lane] * theirs[r];
-                    m[r] = higher;
-                }
-#pragma unroll
-                for (int d = 0; d < kDim / 8; ++d)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) out[d][e] = out[d][e] * mine[e >> 1] + mo[(d * 4 + e) * 32 + lane] * theirs[e >> 1];
-            }
-            asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
-        }
         if (from_start && threadIdx.x == 0)
             p.parts[(int64_t)b * hms + hm] = make_int2((int)blockIdx.x, (int)blockIdx.x + later_parts(u + tiles - 1, share));
-        if (part == 0) {
-            const int slot = from_start ? 1 : 0;
-            const int64_t part_row = ((int64_t)blockIdx.x * 2 + slot) * kRows + rg * 16 + g;
-            float* ml = p.partial + (int64_t)p.ctas * 2 * kRows * kDim;
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                if (!live[r]) continue;
-                const bool any = row_on[r] && l[r] != 0.0f;          // false: the row sees nothing, and is zero whatever V holds
-                const float by = !any ? 0.0f : (whole ? 1.0f / l[r] : 1.0f);
-                if (!whole && c == 0) {
-                    ml[(part_row + 8 * r) * 2] = any ? m[r] : -INFINITY;
-                    ml[(part_row + 8 * r) * 2 + 1] = any ? l[r] : 0.0f;
-                }
-#pragma unroll
-                for (int d = 0; d < kDim / 8; d += (kE4m3 ? 2 : 1)) {
-                    // e4m3: tiles d, d + 1 hold the even and odd columns of chunk d / 2, this thread's are 4 c .. 4 c + 3
-                    const int col = kE4m3 ? 8 * d + 4 * c : 8 * d + 2 * c;
-                    float x[4];
-                    x[0] = out[d][2 * r];
-                    x[1] = kE4m3 ? out[kE4m3 ? d + 1 : d][2 * r] : out[d][2 * r + 1];
-                    x[2] = out[d][2 * r + 1];
-                    x[3] = out[kE4m3 ? d + 1 : d][2 * r + 1];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = any ? x[e] * by : 0.0f;
-                    if (whole) {
-                        T* to = static_cast<T*>(p.o) + o_at[r] + col;
-                        if (kE4m3) {
-                            uint2 w;
-                            w.x = pack2<kTBf16>(x[0], x[1]);
-                            w.y = pack2<kTBf16>(x[2], x[3]);
-                            *reinterpret_cast<uint2*>(to) = w;
-                        } else {
-                            *reinterpret_cast<uint32_t*>(to) = pack2<kTBf16>(x[0], x[1]);
-                        }
-                    } else {
-                        float* to = p.partial + (part_row + 8 * r) * kDim + col;
-                        if (kE4m3) *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
-                        else *reinterpret_cast<float2*>(to) = make_float2(x[0], x[1]);
-                    }
-                }
-            }
-        }
+        const int b_now = b, hm_now = hm;
+        const bool on_now[2] = {row_on[0], row_on[1]};
         u += todo;
         if (tile == tiles) {
             tile = 0;
             u += kBegin;
             if (++hm == hms) { hm = 0; ++b; }
+        }
+        if (u < share.end) fetch();
+
+        // The warps that share a row group put their O side by side, kJoin columns at a time, and each joins and stores its
+        // part of the columns.
+        constexpr int kTiles = S::kJoin / 8;
+        float weight[kSplit][2];
+#pragma unroll
+        for (int h = 0; h < kDim / S::kJoin; ++h) {
+            if (kSplit > 1) {
+                float* ml = merge + kConsumers * 16 * S::kJoin;
+#pragma unroll
+                for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) merge[((warp * kTiles + d) * 4 + e) * 32 + lane] = out[kTiles * h + d][e];
+                if (h == 0 && c == 0) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) { ml[warp * 32 + r * 8 + g] = m[r]; ml[warp * 32 + 16 + r * 8 + g] = l[r]; }
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
+                if (h == 0) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float of[kSplit], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+                        for (int w = 0; w < kSplit; ++w) {
+                            of[w] = ml[(rg * kSplit + w) * 32 + r * 8 + g];
+                            top = fmaxf(top, of[w]);
+                        }
+                        const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                        for (int w = 0; w < kSplit; ++w) {
+                            weight[w][r] = attn_exp2(of[w] - ref);
+                            sum += weight[w][r] * ml[(rg * kSplit + w) * 32 + 16 + r * 8 + g];
+                        }
+                        m[r] = top;
+                        l[r] = sum;
+                    }
+                }
+            }
+            constexpr int kOwn = kTiles / kSplit;           // n-tiles of these columns that this warp stores
+            float x[kOwn][4];
+#pragma unroll
+            for (int d = 0; d < kOwn; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (kSplit == 1) {
+                        x[d][e] = out[kTiles * h + d][e];
+                    } else {
+                        x[d][e] = 0.0f;
+#pragma unroll
+                        for (int w = 0; w < kSplit; ++w)
+                            x[d][e] += merge[(((rg * kSplit + w) * kTiles + part * kOwn + d) * 4 + e) * 32 + lane] * weight[w][e >> 1];
+                    }
+                }
+            // (also before the next queries overwrite these)
+            if (kSplit > 1 || h == 0) asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
+            const int64_t part_row = ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * kRows + rg * 16 + g;
+            float* ml = p.partial + (int64_t)p.ctas * 2 * kRows * kDim;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int head = hm_now / p.row_tiles, row = (hm_now - head * p.row_tiles) * kRows + rg * 16 + g + 8 * r;
+                const int draft = row / p.group;
+                if (draft >= p.drafts) continue;
+                const int64_t o_at = (((int64_t)b_now * p.drafts + draft) * (p.kv_heads * p.group) + head * p.group + row - draft * p.group) * kDim;
+                const bool any = on_now[r] && l[r] != 0.0f;         // false: the row sees nothing, and is zero whatever V holds
+                const float by = !any ? 0.0f : (whole ? 1.0f / l[r] : 1.0f);
+                if (!whole && h == 0 && part == 0 && c == 0) {
+                    ml[(part_row + 8 * r) * 2] = any ? m[r] : -INFINITY;
+                    ml[(part_row + 8 * r) * 2 + 1] = any ? l[r] : 0.0f;
+                }
+#pragma unroll
+                for (int d = 0; d < kOwn; d += (kE4m3 ? 2 : 1)) {
+                    // e4m3: tiles d, d + 1 hold the even and odd columns of a chunk of 16, this thread's are 4 c .. 4 c + 3
+                    const int col = S::kJoin * h + 8 * (part * kOwn + d) + (kE4m3 ? 4 * c : 2 * c);
+                    const int d1 = kE4m3 ? d + 1 : d;
+                    float v[4] = {x[d][2 * r], kE4m3 ? x[d1][2 * r] : x[d][2 * r + 1], x[d][2 * r + 1], x[d1][2 * r + 1]};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = any ? v[e] * by : 0.0f;
+                    if (whole) {
+                        T* to = static_cast<T*>(p.o) + o_at + col;
+                        if (kE4m3) *reinterpret_cast<uint2*>(to) = make_uint2(pack2<kTBf16>(v[0], v[1]), pack2<kTBf16>(v[2], v[3]));
+                        else *reinterpret_cast<uint32_t*>(to) = pack2<kTBf16>(v[0], v[1]);
+                    } else {
+                        float* to = p.partial + (part_row + 8 * r) * kDim + col;
+                        if (kE4m3) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+                        else *reinterpret_cast<float2*>(to) = make_float2(v[0], v[1]);
+                    }
+                }
+            }
         }
     }
     // the join may be scheduled once every CTA is here (it waits for their memory itself)
@@ -688,7 +727,7 @@ int row_groups(int64_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
 template <typename T, bool kE4m3, int kDim, int kGroups>
 int launch_cached(const CachedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t stream) {
     auto kernel = cached_attention_kernel<T, kE4m3, kDim, kGroups>;
-    constexpr int smem = CachedShape<kE4m3, kDim>::kSmem;
+    constexpr int smem = CachedShape<kE4m3, kDim, kGroups>::kSmem;
     if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return BSA_ERR_LAUNCH;
     kernel<<<p.ctas, (kConsumers + 1) * 32, smem, stream>>>(p, map_k, map_v);
     // the join's CTAs may start while the last ones above end; they wait for all of them before they read
