@@ -259,14 +259,15 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
                 m = higher;
                 l *= fall;
                 if (j > 0) {
-#pragma unroll
-                    for (int i = 0; i < kDim / 32; ++i) {
-                        uint32_t acc[32];
-                        tc_ld_32x32b_x32(o_tmem + (uint32_t)(32 * i), acc);
+                    // (rare; 8 columns at a time, beside the 128 scores that are in registers)
+#pragma unroll 1
+                    for (int i = 0; i < kDim; i += 8) {
+                        uint32_t acc[8];
+                        tc_ld_32x32b_x8(o_tmem + (uint32_t)i, acc);
                         tc_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) * fall);
-                        tc_st_32x32b_x32(o_tmem + (uint32_t)(32 * i), acc);
+                        for (int e = 0; e < 8; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) * fall);
+                        tc_st_32x32b_x8(o_tmem + (uint32_t)i, acc);
                     }
                 }
             }
