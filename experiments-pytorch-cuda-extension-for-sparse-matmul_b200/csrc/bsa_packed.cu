@@ -13,9 +13,12 @@
 // 8 x 128 x 128 x D operations, 1024 x D / 64 cycles of the tensor pipe at its peak, and 2 x 128 x 128 exponentials,
 // 2048 cycles of the four MUFU units: at D = 128 the two balance, at D = 64 the exponentials bind.
 //
+// The CTAs are persistent (one per SM, the items in a fixed order that alternates its direction, so that no SM gets the
+// longer one of every round): while the softmax warps end one item, the producer already loads the next one's Q and K and
+// its first scores are computed.
 //   warps 0-3, 4-7   softmax of tile 0 / 1, one row per thread; the epilogue
-//   warp 8           TMA producer: Q, then K and V tiles through a ring of 4 stages
-//   warp 9           MMA issuer: S0 S1 | PV0 S0' PV1 S1' | ..
+//   warp 8           TMA producer: items, Q, then K and V tiles through a ring of 4 stages
+//   warp 9           MMA issuer: S0 S1 | PV0 S0' PV1 S1' | ..; each PV in two parts, the first while the second half of P is made
 // The last K / V tile of a sequence may hold rows of the next one; its V rows are zeroed before use (see zero_rows).
 // All waits are bounded.
 #include "bsa_packed_common.cuh"
@@ -24,24 +27,27 @@ namespace bsa {
 namespace {
 
 constexpr int kFwdStages = 4;
-constexpr int kFwdThreads = 384;                // 10 warps work; 3 warpgroups are needed to hand out registers
+constexpr int kFwdThreads = 320;
+constexpr int kPoly = 0;                        // every kPoly-th pair of exponentials goes to the FMA pipe
 
 struct PackedParams {
     void* o;
     float* lse;                                 // [q_heads, rows], in units of log2, scale included; may be null
     const int32_t* offsets;
     int batch, rows, q_heads, kv_heads, group, causal;
+    int items;                                  // upper bound of the work items
     int pair;                                   // the two tiles: heads 2 h, 2 h + 1 of a group (1), or rows (0)
     float scale_log2;                           // |scale| log2 e
     int negative;                               // scale < 0
     uint32_t* status;
 };
 
-struct __align__(8) FwdBarriers {
-    uint64_t q_full, full[kFwdStages], empty[kFwdStages];
-    uint64_t s_full[2], p_full[2], o_full[2];
+struct __align__(16) FwdBarriers {
+    uint64_t item_full[2], item_empty[2];
+    uint64_t q_full[2], q_empty[2], full[kFwdStages], empty[kFwdStages];
+    uint64_t s_full[2], p_full[2][2], o_full[2];
     uint64_t drain;
-    PackedItem item;
+    int4 items[2];                              // first row of the sequence, its length, the tile, the first head; length 0: no more
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -49,148 +55,187 @@ struct __align__(8) FwdBarriers {
 template <int kDim>
 constexpr int fwd_smem() { return (2 + kFwdStages) * (kDim / 64) * kPanelBytes + (int)sizeof(FwdBarriers); }
 
+// What an item means: K / V tiles of each of its two Q tiles.
+struct FwdItem {
+    int start, length, row0, head0, steps[2];
+    __device__ __forceinline__ FwdItem(const int4& v, const PackedParams& p) {
+        start = v.x; length = v.y; head0 = v.w;
+        row0 = v.z * (p.pair ? kRowsTile : 2 * kRowsTile);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int first = p.pair ? row0 : row0 + s * kRowsTile;
+            const int keys = p.causal ? min(first + kRowsTile, length) : length;
+            steps[s] = first < length ? (keys + kRowsTile - 1) / kRowsTile : 0;
+        }
+    }
+};
+
 template <bool kBf16, int kDim>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap map_q,
                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
-    constexpr int kPanels = kDim / 64, kTileBytes_ = kPanels * kPanelBytes;
+    constexpr int kPanels = kDim / 64, kTile_ = kPanels * kPanelBytes;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t* ring = smem + 2 * kTileBytes_;
-    FwdBarriers* bars = reinterpret_cast<FwdBarriers*>(ring + kFwdStages * kTileBytes_);
+    uint8_t* ring = smem + 2 * kTile_;
+    FwdBarriers* bars = reinterpret_cast<FwdBarriers*>(ring + kFwdStages * kTile_);
     int* abort_flag = &bars->abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per_tile = p.pair ? kRowsTile : 2 * kRowsTile;
-    const int head_items = p.pair ? p.q_heads / 2 : p.q_heads;
-    const int rank = (int)blockIdx.x / head_items, head_item = (int)blockIdx.x - rank * head_items;
 
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(&bars->tmem_base)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (warp == 8) {
-        const PackedItem found = packed_locate(p.offsets, p.batch, p.rows, per_tile, rank, lane, p.status);
-        if (lane == 0) {
-            bars->item = found;
-            *abort_flag = 0;
-            mbar_init(&bars->q_full, 1);
-            for (int i = 0; i < kFwdStages; ++i) { mbar_init(&bars->full[i], 1); mbar_init(&bars->empty[i], 1); }
-            for (int i = 0; i < 2; ++i) { mbar_init(&bars->s_full[i], 1); mbar_init(&bars->p_full[i], 128); mbar_init(&bars->o_full[i], 1); }
-            mbar_init(&bars->drain, 1);
-            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-            fence_async_shared();
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int i = 0; i < kFwdStages; ++i) { mbar_init(&bars->full[i], 1); mbar_init(&bars->empty[i], 1); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars->item_full[i], 1); mbar_init(&bars->item_empty[i], 9);
+            mbar_init(&bars->q_full[i], 1); mbar_init(&bars->q_empty[i], 1);
+            mbar_init(&bars->s_full[i], 1); mbar_init(&bars->o_full[i], 1);
+            mbar_init(&bars->p_full[i][0], 4); mbar_init(&bars->p_full[i][1], 4);
         }
+        mbar_init(&bars->drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_shared();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t*)&bars->tmem_base;
-    const PackedItem item = bars->item;
-    const int head0 = p.pair ? 2 * head_item : head_item;       // tile s: head head0 + s (pair) or rows + 128 s
-    const int tiles = (item.length + per_tile - 1) / per_tile;
-    // the later tiles of a causal sequence are the longer ones: they go first
-    const int tile = tiles - 1 - item.tile;
-    const int row0 = tile * per_tile;                           // in the sequence
-    const bool work = item.length > 0 && item.b < p.batch;
-    // K / V tiles of each Q tile
-    int steps[2] = {0, 0};
-    if (work) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int first = p.pair ? row0 : row0 + s * kRowsTile;
-            if (first < item.length) {
-                const int keys = p.causal ? min(first + kRowsTile, item.length) : item.length;
-                steps[s] = (keys + kRowsTile - 1) / kRowsTile;
-            }
-        }
-    }
-    const int all_steps = max(steps[0], steps[1]);
-    const uint32_t fmt = kBf16 ? 1u : 0u;
-    const uint32_t common = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kRowsTile >> 4) << 24);
+    bool ok = true;
+    // the next item, for every warp but the producer; false: no more
+    int item_no = 0;
+    auto next_item = [&](int4& v) {
+        const int slot = item_no & 1;
+        ok = wait_all(&bars->item_full[slot], (uint32_t)(item_no >> 1) & 1u, abort_flag, p.status);
+        if (!ok) return false;
+        v = bars->items[slot];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->item_empty[slot]);
+        ++item_no;
+        return v.y > 0;
+    };
 
-    if (item.length > 0 && item.b == p.batch) {                 // rows behind the last sequence
-        const int from = item.start + item.tile * per_tile, to = min(from + per_tile, p.rows);
-        for (int h = head0; h <= head0 + p.pair; ++h) {
-            zero_tail(p.o, from, to, h, p.q_heads, kDim);
-            if (p.lse)
-                for (int r = from + (int)threadIdx.x; r < to; r += blockDim.x) p.lse[(size_t)h * p.rows + r] = -INFINITY;
-        }
-    }
     if (warp == 8) {
         // ------------------------------------------------------------ producer
-        if (all_steps > 0) {
-            const int kv_head = head0 / p.group;
-            bool ok = true;
+        const int per_tile = p.pair ? kRowsTile : 2 * kRowsTile;
+        const int head_items = p.pair ? p.q_heads / 2 : p.q_heads, ctas = (int)gridDim.x;
+        int posted = 0, t = 0, q_no[2] = {0, 0};
+        auto post = [&](const int4& v) {
+            const int slot = posted & 1;
+            ok = wait_all(&bars->item_empty[slot], ((uint32_t)(posted >> 1) & 1u) ^ 1u, abort_flag, p.status);
+            if (ok && lane == 0) {
+                bars->items[slot] = v;
+                mbar_arrive(&bars->item_full[slot]);
+            }
+            __syncwarp();
+            ++posted;
+        };
+        auto load = [&](uint8_t* to, const CUtensorMap* map, uint64_t* bar, int head, int row) {
             if (elect_one()) {
-                mbar_expect_tx(&bars->q_full, (uint32_t)(2 * kTileBytes_));
+                mbar_expect_tx(bar, (uint32_t)kTile_);
 #pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int c = 0; c < kPanels; ++c)
-                        tma_load_3d(smem + s * kTileBytes_ + c * kPanelBytes, &map_q, &bars->q_full, 64 * c,
-                                    p.pair ? head0 + s : head0, item.start + row0 + (p.pair ? 0 : s * kRowsTile));
+                for (int c = 0; c < kPanels; ++c) tma_load_3d(to + c * kPanelBytes, map, bar, 64 * c, head, row);
             }
             __syncwarp();
-            for (int t = 0; ok && t < 2 * all_steps; ++t) {     // K of step t / 2, then V
-                const int stage = t % kFwdStages;
-                ok = __all_sync(0xffffffffu, mbar_wait(&bars->empty[stage], ((uint32_t)(t / kFwdStages) & 1u) ^ 1u, abort_flag, p.status)) != 0;
-                if (ok && elect_one()) {
-                    mbar_expect_tx(&bars->full[stage], (uint32_t)kTileBytes_);
-                    const CUtensorMap* map = t & 1 ? &map_v : &map_k;
-#pragma unroll
-                    for (int c = 0; c < kPanels; ++c)
-                        tma_load_3d(ring + stage * kTileBytes_ + c * kPanelBytes, map, &bars->full[stage], 64 * c, kv_head,
-                                    item.start + (t / 2) * kRowsTile);
+        };
+        for (int round = 0; ok && (int64_t)round * ctas < p.items; ++round) {
+            const int64_t at = (int64_t)round * ctas + (round & 1 ? ctas - 1 - (int)blockIdx.x : (int)blockIdx.x);
+            if (at >= p.items) continue;
+            const int rank = (int)(at / head_items), head_item = (int)at - rank * head_items, head0 = p.pair ? 2 * head_item : head_item;
+            PackedItem found = packed_locate(p.offsets, p.batch, p.rows, per_tile, rank, lane, p.status);
+            if (found.length == 0) continue;
+            if (found.b == p.batch) {                           // rows behind the last sequence
+                const int from = found.start + found.tile * per_tile, to = min(from + per_tile, p.rows);
+                for (int h = head0; h <= head0 + p.pair; ++h) {
+                    zero_tail(p.o, from, to, h, p.q_heads, kDim, lane, 32);
+                    if (p.lse)
+                        for (int r = from + lane; r < to; r += 32) p.lse[(size_t)h * p.rows + r] = -INFINITY;
                 }
-                __syncwarp();
+                continue;
             }
-            if (lane == 0 && *(volatile int*)abort_flag) let_copies_land();
-            __syncwarp();
+            const int4 v = make_int4(found.start, found.length, found.tile, head0);
+            post(v);
+            const FwdItem item(v, p);
+            const int all_steps = max(item.steps[0], item.steps[1]), kv_head = head0 / p.group;
+            for (int j = 0; ok && j < 2 * all_steps; ++j, ++t) {        // K of step j / 2, then V; the Q tiles around the first
+                if (j < 2 && item.steps[j] > 0) {
+                    ok = wait_all(&bars->q_empty[j], ((uint32_t)q_no[j] & 1u) ^ 1u, abort_flag, p.status);
+                    if (!ok) break;
+                    ++q_no[j];
+                    load(smem + j * kTile_, &map_q, &bars->q_full[j], p.pair ? head0 + j : head0,
+                         item.start + item.row0 + (p.pair ? 0 : j * kRowsTile));
+                }
+                const int stage = t % kFwdStages;
+                ok = wait_all(&bars->empty[stage], ((uint32_t)(t / kFwdStages) & 1u) ^ 1u, abort_flag, p.status);
+                if (ok) load(ring + stage * kTile_, j & 1 ? &map_v : &map_k, &bars->full[stage], kv_head, item.start + (j / 2) * kRowsTile);
+            }
         }
+        if (ok) post(make_int4(0, 0, 0, 0));
+        if (lane == 0 && *(volatile int*)abort_flag) let_copies_land();
+        __syncwarp();
     } else if (warp == 9) {
         // ------------------------------------------------------------ MMA issuer
-        if (all_steps > 0) {
-            const uint32_t idesc_s = common | ((uint32_t)(kRowsTile >> 3) << 17);
-            const uint32_t idesc_o = common | (1u << 16) | ((uint32_t)(kDim >> 3) << 17);
-            const uint64_t q_desc[2] = {panel_desc(smem_u32(smem), false), panel_desc(smem_u32(smem + kTileBytes_), false)};
-            bool ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_full, 0, abort_flag, p.status)) != 0;
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bars->full[0], 0, abort_flag, p.status)) != 0;
-            if (ok) {
-                tc_fence_after();
-                const uint64_t k_desc = panel_desc(smem_u32(ring), false);
-                if (elect_one()) {
-#pragma unroll
-                    for (int s = 0; s < 2; ++s)
-                        if (steps[s] > 0) {
-                            mma_rows<kDim>(tmem + (uint32_t)(s * 128), q_desc[s], k_desc, idesc_s);
-                            tc_commit(&bars->s_full[s]);
-                        }
-                    tc_commit(&bars->empty[0]);
-                }
-                __syncwarp();
-            }
-            for (int j = 0; ok && j < all_steps; ++j) {
-                const int v_no = 2 * j + 1, k_no = 2 * j + 2, v_stage = v_no % kFwdStages, k_stage = k_no % kFwdStages;
-                const bool more = j + 1 < all_steps;
-                ok = __all_sync(0xffffffffu, mbar_wait(&bars->full[v_stage], (uint32_t)(v_no / kFwdStages) & 1u, abort_flag, p.status)) != 0;
-                if (ok && more)
-                    ok = __all_sync(0xffffffffu, mbar_wait(&bars->full[k_stage], (uint32_t)(k_no / kFwdStages) & 1u, abort_flag, p.status)) != 0;
-                if (!ok) break;
-                const int valid = item.length - j * kRowsTile;
-                if (valid < kRowsTile) zero_rows<kDim>(ring + v_stage * kTileBytes_, valid, lane);
-                const uint64_t v_desc = panel_desc(smem_u32(ring + v_stage * kTileBytes_), true);
-                const uint64_t k_desc = panel_desc(smem_u32(ring + k_stage * kTileBytes_), false);
+        const uint32_t fmt = kBf16 ? 1u : 0u;
+        const uint32_t common = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kRowsTile >> 4) << 24);
+        const uint32_t idesc_s = common | ((uint32_t)(kRowsTile >> 3) << 17);
+        const uint32_t idesc_o = common | (1u << 16) | ((uint32_t)(kDim >> 3) << 17);
+        const uint64_t q_desc[2] = {panel_desc(smem_u32(smem), false), panel_desc(smem_u32(smem + kTile_), false)};
+        int t = 0, q_no[2] = {0, 0}, p_no[2] = {0, 0};          // tiles of the ring, Q tiles and P tiles so far
+        auto stage_ready = [&](int no) {
+            ok = wait_all(&bars->full[no % kFwdStages], (uint32_t)(no / kFwdStages) & 1u, abort_flag, p.status);
+            return ok;
+        };
+        int4 v;
+        while (next_item(v)) {
+            const FwdItem item(v, p);
+            const int all_steps = max(item.steps[0], item.steps[1]);
+            if (!stage_ready(t)) break;
+            {
+                const uint64_t k_desc = panel_desc(smem_u32(ring + t % kFwdStages * kTile_), false);
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    if (!ok || j >= steps[s]) continue;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_full[s], (uint32_t)j & 1u, abort_flag, p.status)) != 0;
+                    if (!ok || item.steps[s] == 0) continue;
+                    ok = wait_all(&bars->q_full[s], (uint32_t)q_no[s]++ & 1u, abort_flag, p.status);
                     if (!ok) continue;
                     tc_fence_after();
                     if (elect_one()) {
-                        mma_keys(tmem + (uint32_t)(256 + s * kDim), tmem + (uint32_t)(s * 128), v_desc, idesc_o, j > 0);
-                        if (j + 1 < steps[s]) {
-                            mma_rows<kDim>(tmem + (uint32_t)(s * 128), q_desc[s], k_desc, idesc_s);
+                        mma_rows<kDim>(tmem + (uint32_t)(s * 128), q_desc[s], k_desc, idesc_s);
+                        tc_commit(&bars->s_full[s]);
+                        if (item.steps[s] == 1) tc_commit(&bars->q_empty[s]);
+                    }
+                    __syncwarp();
+                }
+                if (ok && elect_one()) tc_commit(&bars->empty[t % kFwdStages]);
+                __syncwarp();
+            }
+            for (int j = 0; ok && j < all_steps; ++j) {
+                const int v_stage = (t + 2 * j + 1) % kFwdStages, k_stage = (t + 2 * j + 2) % kFwdStages;
+                const bool more = j + 1 < all_steps;
+                if (!stage_ready(t + 2 * j + 1) || (more && !stage_ready(t + 2 * j + 2))) break;
+                const int valid = item.length - j * kRowsTile;
+                if (valid < kRowsTile) zero_rows<kDim>(ring + v_stage * kTile_, valid, lane);
+                const uint64_t v_desc = panel_desc(smem_u32(ring + v_stage * kTile_), true);
+                const uint64_t k_desc = panel_desc(smem_u32(ring + k_stage * kTile_), false);
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    if (!ok || j >= item.steps[s]) continue;
+                    const uint32_t s_tmem = tmem + (uint32_t)(s * 128), o_tmem = tmem + (uint32_t)(256 + s * kDim);
+                    ok = wait_all(&bars->p_full[s][0], (uint32_t)p_no[s] & 1u, abort_flag, p.status);
+                    if (!ok) continue;
+                    tc_fence_after();
+                    if (elect_one()) mma_keys<0>(o_tmem, s_tmem, v_desc, idesc_o, j > 0);
+                    __syncwarp();
+                    ok = wait_all(&bars->p_full[s][1], (uint32_t)p_no[s]++ & 1u, abort_flag, p.status);
+                    if (!ok) continue;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        mma_keys<1>(o_tmem, s_tmem, v_desc, idesc_o, true);
+                        if (j + 1 < item.steps[s]) {
+                            mma_rows<kDim>(s_tmem, q_desc[s], k_desc, idesc_s);
                             tc_commit(&bars->s_full[s]);
+                            if (j + 2 == item.steps[s]) tc_commit(&bars->q_empty[s]);
                         } else {
                             tc_commit(&bars->o_full[s]);
                         }
@@ -203,107 +248,126 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
                 }
                 __syncwarp();
             }
-            // all MMAs issued by the elected lane must have retired before TMEM is freed
-            if (elect_one()) {
-                tc_commit(&bars->drain);
-                mbar_wait(&bars->drain, 0, abort_flag, p.status);
-            }
-            __syncwarp();
+            t += 2 * all_steps;
+            if (!ok) break;
         }
-    } else if (warp < 8) {
+        // all MMAs issued by the elected lane must have retired before TMEM is freed
+        if (elect_one()) {
+            tc_commit(&bars->drain);
+            mbar_wait(&bars->drain, 0, abort_flag, p.status);
+        }
+        __syncwarp();
+    } else {
         // ------------------------------------------------------------ softmax of tile s, one row per thread
         const int s = warp >> 2, r = (warp & 3) * 32 + lane;
-        const int n = steps[s];
-        const int row = row0 + (p.pair ? 0 : s * kRowsTile) + r;        // in the sequence
-        const int last = p.causal ? min(row, item.length - 1) : item.length - 1;      // the last key the row sees
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_tmem = tmem + lanes + (uint32_t)(s * 128), o_tmem = tmem + lanes + (uint32_t)(256 + s * kDim);
         const float c = p.scale_log2;
-        float m = -INFINITY, l = 0.0f;                                  // m in units of c S
-        bool ok = true;
-        for (int j = 0; ok && j < n; ++j) {
-            ok = mbar_wait(&bars->s_full[s], (uint32_t)j & 1u, abort_flag, p.status);
-            ok = __all_sync(0xffffffffu, ok) != 0;
-            if (!ok) break;
-            tc_fence_after();
-            uint32_t x[4][32];
+        int s_no = 0, o_no = 0;
+        int4 v;
+        while (next_item(v)) {
+            const FwdItem item(v, p);
+            const int n = item.steps[s];
+            if (n == 0) continue;
+            const int row = item.row0 + (p.pair ? 0 : s * kRowsTile) + r;           // in the sequence
+            const int last = p.causal ? min(row, item.length - 1) : item.length - 1;      // the last key the row sees
+            float m = -INFINITY, l = 0.0f;                                          // m in units of c S
+            for (int j = 0; j < n; ++j) {
+                ok = wait_all(&bars->s_full[s], (uint32_t)s_no++ & 1u, abort_flag, p.status);
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t x[4][32];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tc_ld_32x32b_x32(s_tmem + (uint32_t)(32 * i), x[i]);
-            tc_wait_ld();
-            if (p.negative) {
+                for (int i = 0; i < 4; ++i) tc_ld_32x32b_x32(s_tmem + (uint32_t)(32 * i), x[i]);
+                tc_wait_ld();
+                if (p.negative) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) x[i][e] ^= 0x80000000u;
-            }
-            const int see = last - j * kRowsTile;                       // columns 0 .. see of the tile are seen
-            if (__any_sync(0xffffffffu, see < kRowsTile - 1)) {
+                        for (int e = 0; e < 32; ++e) x[i][e] ^= 0x80000000u;
+                }
+                const int see = last - j * kRowsTile;                               // columns 0 .. see of the tile are seen
+                const bool masked = __any_sync(0xffffffffu, see < kRowsTile - 1) != 0;
+                if (masked) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (32 * i + e > see) x[i][e] = 0xff800000u;
-            }
-            float top[4];
+                        for (int e = 0; e < 32; ++e)
+                            if (32 * i + e > see) x[i][e] = 0xff800000u;
+                }
+                float top[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                top[i] = __uint_as_float(x[i][0]);
+                for (int i = 0; i < 4; ++i) {
+                    top[i] = __uint_as_float(x[i][0]);
 #pragma unroll
-                for (int e = 1; e < 31; e += 2) top[i] = fmax3(top[i], __uint_as_float(x[i][e]), __uint_as_float(x[i][e + 1]));
-                top[i] = fmaxf(top[i], __uint_as_float(x[i][31]));
-            }
-            const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-            if (__any_sync(0xffffffffu, mt > m + 8.0f)) {
-                const float higher = fmaxf(m, mt);
-                const float fall = higher == -INFINITY ? 1.0f : attn_exp2(m - higher);
-                m = higher;
-                l *= fall;
-                if (j > 0) {
-                    // (rare; 8 columns at a time, beside the 128 scores that are in registers)
+                    for (int e = 1; e < 31; e += 2) top[i] = fmax3(top[i], __uint_as_float(x[i][e]), __uint_as_float(x[i][e + 1]));
+                    top[i] = fmaxf(top[i], __uint_as_float(x[i][31]));
+                }
+                const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+                if (__any_sync(0xffffffffu, mt > m + 8.0f)) {
+                    const float higher = fmaxf(m, mt);
+                    const float fall = higher == -INFINITY ? 1.0f : attn_exp2(m - higher);
+                    m = higher;
+                    l *= fall;
+                    if (j > 0) {
+                        // rare; 8 columns at a time, beside the 128 scores that are in registers
 #pragma unroll 1
-                    for (int i = 0; i < kDim; i += 8) {
-                        uint32_t acc[8];
-                        tc_ld_32x32b_x8(o_tmem + (uint32_t)i, acc);
-                        tc_wait_ld();
+                        for (int i = 0; i < kDim; i += 8) {
+                            uint32_t acc[8];
+                            tc_ld_32x32b_x8(o_tmem + (uint32_t)i, acc);
+                            tc_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) * fall);
-                        tc_st_32x32b_x8(o_tmem + (uint32_t)i, acc);
+                            for (int e = 0; e < 8; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) * fall);
+                            tc_st_32x32b_x8(o_tmem + (uint32_t)i, acc);
+                        }
                     }
                 }
-            }
-            const float ref = m == -INFINITY ? 0.0f : -m;
-            float sum[2] = {0.0f, 0.0f};
+                const float ref = m == -INFINITY ? 0.0f : -m;
+                const uint64_t c2 = f2_pack(c, c), ref2 = f2_pack(ref, ref);
+                uint64_t sum[2] = {0ull, 0ull};
+                // The first half of P goes out before the second is made: its products run meanwhile.
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+                for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    const float a = attn_exp2(fmaf(__uint_as_float(x[i][e]), c, ref));
-                    const float b = attn_exp2(fmaf(__uint_as_float(x[i][e + 1]), c, ref));
-                    sum[0] += a;
-                    sum[1] += b;
-                    x[i / 2][(i & 1) * 16 + e / 2] = pack2<kBf16>(a, b);
+                    for (int i = 2 * half; i < 2 * half + 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            const uint64_t y = f2_fma(f2_pack(__uint_as_float(x[i][e]), __uint_as_float(x[i][e + 1])), c2, ref2);
+                            float a, b;
+                            if (kPoly > 0 && (e / 2) % (kPoly > 0 ? kPoly : 1) == 1 && !masked) {
+                                exp2_pair(y, a, b);
+                            } else {
+                                f2_unpack(y, a, b);
+                                a = attn_exp2(a);
+                                b = attn_exp2(b);
+                            }
+                            sum[(e / 2) & 1] = f2_add(sum[(e / 2) & 1], f2_pack(a, b));
+                            x[half][(i & 1) * 16 + e / 2] = pack2<kBf16>(a, b);
+                        }
+                    tc_st_32x32b_x32(s_tmem + (uint32_t)(32 * half), x[half]);
+                    tc_wait_st();
+                    arrive_warp(&bars->p_full[s][half], lane);
                 }
-                if (i & 1) tc_st_32x32b_x32(s_tmem + (uint32_t)(32 * (i / 2)), x[i / 2]);
+                float a, b;
+                f2_unpack(f2_add(sum[0], sum[1]), a, b);
+                l += a + b;
             }
-            l += sum[0] + sum[1];
-            tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(&bars->p_full[s]);
-        }
-        if (n > 0) {
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[s], 0, abort_flag, p.status)) != 0;
+            if (!ok) break;
+            ok = wait_all(&bars->o_full[s], (uint32_t)o_no++ & 1u, abort_flag, p.status);
+            if (!ok) break;
             tc_fence_after();
-            const int head = p.pair ? head0 + s : head0;
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            uint8_t* to = static_cast<uint8_t*>(p.o) + (((size_t)(item.start + row) * p.q_heads + head) * kDim) * 2;
+            uint32_t acc[kDim / 32][32];
 #pragma unroll
-            for (int i = 0; i < kDim / 32; ++i) {
-                uint32_t acc[32];
-                tc_ld_32x32b_x32(o_tmem + (uint32_t)(32 * i), acc);
-                tc_wait_ld();
-                if (ok && row < item.length) store_row32<kBf16>(to + 64 * i, acc, inv);
+            for (int i = 0; i < kDim / 32; ++i) tc_ld_32x32b_x32(o_tmem + (uint32_t)(32 * i), acc[i]);
+            tc_wait_ld();
+            const int head = p.pair ? item.head0 + s : item.head0;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            if (row < item.length) {
+                uint8_t* to = static_cast<uint8_t*>(p.o) + (((size_t)(item.start + row) * p.q_heads + head) * kDim) * 2;
+#pragma unroll
+                for (int i = 0; i < kDim / 32; ++i) store_row32<kBf16>(to + 64 * i, acc[i], inv);
+                if (p.lse) p.lse[(size_t)head * p.rows + item.start + row] = m + __log2f(l);
             }
-            if (ok && row < item.length && p.lse) p.lse[(size_t)head * p.rows + item.start + row] = m + __log2f(l);
         }
     }
     tc_fence_before();
@@ -316,14 +380,16 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
 }
 
 template <bool kBf16, int kDim>
-int launch_forward(const PackedParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
+int launch_forward(PackedParams p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
     auto kernel = packed_forward_kernel<kBf16, kDim>;
     constexpr int smem = fwd_smem<kDim>();
     if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return BSA_ERR_LAUNCH;
     // an upper bound of the tiles: every sequence and the rows behind the last one may end inside a tile
     const int per_tile = p.pair ? kRowsTile : 2 * kRowsTile;
-    const unsigned grid = (unsigned)((p.rows / per_tile + p.batch + 1) * (p.pair ? p.q_heads / 2 : p.q_heads));
-    kernel<<<grid, kFwdThreads, smem, stream>>>(p, mq, mk, mv);
+    p.items = (p.rows / per_tile + p.batch + 1) * (p.pair ? p.q_heads / 2 : p.q_heads);
+    const int sms = sm_count();
+    if (sms <= 0) return BSA_ERR_LAUNCH;
+    kernel<<<p.items < sms ? p.items : sms, kFwdThreads, smem, stream>>>(p, mq, mk, mv);
     return launch_status();
 }
 

@@ -124,14 +124,6 @@ __device__ __forceinline__ void bwd_end(uint32_t tmem, int warp) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
-__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, int* abort_flag, uint32_t* status) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status)) != 0;
-}
-__device__ __forceinline__ void arrive_warp(uint64_t* bar, int lane) {
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar);
-}
 template <int kDim>
 __device__ __forceinline__ void load_tile(uint8_t* to, const CUtensorMap* map, uint64_t* bar, int head, int row) {
 #pragma unroll
@@ -158,14 +150,15 @@ packed_keys_kernel(const PackedBwdParams p, const __grid_constant__ CUtensorMap 
     const PackedItem item = bars->item;
     const bool work = item.length > 0 && item.b < p.batch;
     const int tiles = (item.length + kRowsTile - 1) / kRowsTile;
-    const int first_q = p.causal ? item.tile : 0;               // the query tiles that see these keys: first_q .. tiles - 1
+    const int key_tile = tiles - 1 - item.tile;                 // (the first keys are seen by the most queries)
+    const int first_q = p.causal ? key_tile : 0;                // the query tiles that see these keys: first_q .. tiles - 1
     const int per_head = tiles - first_q, n = work ? per_head * p.group : 0;
     const uint32_t s_tmem = tmem, dp_tmem = tmem + 128u, dv_tmem = tmem + 256u, dk_tmem = tmem + 256u + kDim;
 
     if (item.length > 0 && item.b == p.batch) {                 // rows behind the last sequence
         const int from = item.start + item.tile * kRowsTile, to = min(from + kRowsTile, p.rows);
-        zero_tail(p.dk, from, to, kv_head, p.kv_heads, kDim);
-        zero_tail(p.dv, from, to, kv_head, p.kv_heads, kDim);
+        zero_tail(p.dk, from, to, kv_head, p.kv_heads, kDim, threadIdx.x, blockDim.x);
+        zero_tail(p.dv, from, to, kv_head, p.kv_heads, kDim, threadIdx.x, blockDim.x);
     }
     if (warp == 8) {
         // ------------------------------------------------------------ producer
@@ -173,8 +166,8 @@ packed_keys_kernel(const PackedBwdParams p, const __grid_constant__ CUtensorMap 
             bool ok = true;
             if (elect_one()) {
                 mbar_expect_tx(&bars->x_full, (uint32_t)(2 * kTile_));
-                load_tile<kDim>(k_smem, &map_k, &bars->x_full, kv_head, item.start + item.tile * kRowsTile);
-                load_tile<kDim>(v_smem, &map_v, &bars->x_full, kv_head, item.start + item.tile * kRowsTile);
+                load_tile<kDim>(k_smem, &map_k, &bars->x_full, kv_head, item.start + key_tile * kRowsTile);
+                load_tile<kDim>(v_smem, &map_v, &bars->x_full, kv_head, item.start + key_tile * kRowsTile);
             }
             __syncwarp();
             int head = kv_head * p.group, qt = first_q;
@@ -294,7 +287,7 @@ packed_keys_kernel(const PackedBwdParams p, const __grid_constant__ CUtensorMap 
             const int st = i & 1;
             const float4* stat = st_smem + st * (kRowsTile / 2) + 32 * half;
             // columns (queries of this half) from `from` up to `to` see the key
-            const int from = (p.causal && qt == item.tile ? r : 0) - 64 * half, to = item.length - qt * kRowsTile - 64 * half;
+            const int from = (p.causal && qt == key_tile ? r : 0) - 64 * half, to = item.length - qt * kRowsTile - 64 * half;
             const bool masked = __any_sync(0xffffffffu, from > 0 || to < 64) != 0;
             ok = ok && wait_all(&bars->st_full[st], (uint32_t)(i >> 1) & 1u, abort_flag, p.status);
             ok = ok && wait_all(&bars->s_full[0], (uint32_t)i & 1u, abort_flag, p.status);
@@ -348,7 +341,7 @@ packed_keys_kernel(const PackedBwdParams p, const __grid_constant__ CUtensorMap 
         }
         ok = ok && wait_all(&bars->done, 0, abort_flag, p.status);
         tc_fence_after();
-        const int key = item.tile * kRowsTile + r;
+        const int key = key_tile * kRowsTile + r;
         const size_t at = ((size_t)(item.start + key) * p.kv_heads + kv_head) * kDim;
 #pragma unroll
         for (int i = 0; i < kDim / 64; ++i) {                   // this half's columns of both
@@ -384,13 +377,13 @@ packed_queries_kernel(const PackedBwdParams p, const __grid_constant__ CUtensorM
     const PackedItem item = bars->item;
     const bool work = item.length > 0 && item.b < p.batch;
     const int tiles = (item.length + kRowsTile - 1) / kRowsTile;
-    const int tile = tiles - 1 - item.tile;                     // the longer ones first
+    const int tile = item.tile;
     const int n = work ? (p.causal ? tile + 1 : tiles) : 0;
     const uint32_t dp_tmem = tmem + 256u, dq_tmem = tmem + 384u;
 
     if (item.length > 0 && item.b == p.batch) {
         const int from = item.start + item.tile * kRowsTile, to = min(from + kRowsTile, p.rows);
-        zero_tail(p.dq, from, to, head, p.q_heads, kDim);
+        zero_tail(p.dq, from, to, head, p.q_heads, kDim, threadIdx.x, blockDim.x);
     }
     if (warp == 8) {
         // ------------------------------------------------------------ producer

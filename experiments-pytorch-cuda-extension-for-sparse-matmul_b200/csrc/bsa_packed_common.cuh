@@ -15,41 +15,69 @@ struct PackedItem {
     int start, length, tile, b;                             // first row and rows of the sequence; length 0: nothing to do
 };
 
-// Item `rank` of the list of all tiles: the sequences in order, `per_tile` rows per tile, then the rows behind the last
-// sequence.  Called by one warp; nothing about the offsets is known on the host.  Offsets that are not
-// 0 <= o_0 = 0 <= o_1 <= .. <= rows are reported, and clamped so that nothing outside the tensors is touched.
+__device__ __forceinline__ int warp_sum(int x) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+}
+// Item `rank` of the list of all tiles of `per_tile` rows, called by one warp; nothing about the offsets is known on the
+// host.  The list goes by the number of a tile in its sequence, the largest first (of a causal sequence the later tiles
+// are the longer ones, so this is longest first over all sequences), and by the sequence's number among equals; the tiles of the
+// rows behind the last sequence come last.  F(t) = sum_b max(0, tiles_b - t) items have a number of t or more, so the
+// item's number is the largest t with F(t) > rank, found by bisection.
+// Offsets that are not 0 = o_0 <= o_1 <= .. <= rows are reported, and clamped so that nothing outside the tensors is
+// touched.
 __device__ __forceinline__ PackedItem packed_locate(const int32_t* offsets, int batch, int rows, int per_tile, int rank,
                                                     int lane, uint32_t* status) {
-    int before = 0;
-    for (int b0 = 0; b0 <= batch; b0 += 32) {
-        const int b = b0 + lane;
-        int start = 0, end = 0;
-        if (b <= batch) {
-            const int from = offsets[b], to = b < batch ? offsets[b + 1] : rows;
-            start = min(max(from, 0), rows);
-            end = min(max(to, start), rows);
-            if (from != start || to != end || (b == 0 && from != 0)) atomicExch(status, (uint32_t)BSA_ERR_BAD_SHAPE);
-        }
-        const int tiles = (end - start + per_tile - 1) / per_tile;
-        int upto = tiles;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += o;
-        }
-        const uint32_t past = __ballot_sync(0xffffffffu, rank < before + upto);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            PackedItem item;
-            item.start = __shfl_sync(0xffffffffu, start, l);
-            item.length = __shfl_sync(0xffffffffu, end, l) - item.start;
-            item.tile = rank - before - __shfl_sync(0xffffffffu, upto - tiles, l);
-            item.b = b0 + l;
-            return item;
-        }
-        before += __shfl_sync(0xffffffffu, upto, 31);
+    const auto span = [&](int b, int& start) {              // rows of sequence b
+        start = 0;
+        if (b >= batch) return 0;
+        start = min(max(offsets[b], 0), rows);
+        return min(max(offsets[b + 1], start), rows) - start;
+    };
+    int most = 0, all = 0;
+    for (int b = lane; b < batch; b += 32) {
+        int start;
+        const int length = span(b, start), tiles = (length + per_tile - 1) / per_tile;
+        if (offsets[b] != start || offsets[b + 1] != start + length || (b == 0 && start != 0)) atomicExch(status, (uint32_t)BSA_ERR_BAD_SHAPE);
+        most = max(most, tiles);
+        all += tiles;
     }
-    return PackedItem{0, 0, 0, 0};
+    most = (int)__reduce_max_sync(0xffffffffu, (uint32_t)most);
+    all = warp_sum(all);
+    PackedItem item{0, 0, 0, 0};
+    if (rank >= all) {
+        const int behind = min(max(offsets[batch], 0), rows);
+        if (rank - all < (rows - behind + per_tile - 1) / per_tile) item = PackedItem{behind, rows - behind, rank - all, batch};
+        return item;
+    }
+    int t = 0, end = most, above = 0;                       // F(t) > rank >= F(end) = above
+    while (end - t > 1) {
+        const int mid = (t + end) / 2;
+        int f = 0;
+        for (int b = lane; b < batch; b += 32) {
+            int start;
+            f += max((span(b, start) + per_tile - 1) / per_tile - mid, 0);
+        }
+        f = warp_sum(f);
+        if (f > rank) t = mid;
+        else { end = mid; above = f; }
+    }
+    int nth = rank - above;                                 // among the sequences that have a tile t
+    for (int b0 = 0; b0 < batch; b0 += 32) {
+        int start;
+        const int length = span(b0 + lane, start);
+        uint32_t has = __ballot_sync(0xffffffffu, (length + per_tile - 1) / per_tile > t);
+        if (nth >= __popc(has)) { nth -= __popc(has); continue; }
+        for (; nth > 0; --nth) has &= has - 1;
+        const int l = __ffs(has) - 1;
+        item.start = __shfl_sync(0xffffffffu, start, l);
+        item.length = __shfl_sync(0xffffffffu, length, l);
+        item.tile = t;
+        item.b = b0 + l;
+        break;
+    }
+    return item;
 }
 
 // Operand descriptor of a 128-row tile in 64-element panels: K-major (a row is one M / N index) or MN-major (a row is
@@ -72,13 +100,24 @@ __device__ __forceinline__ void mma_rows(uint32_t tmem_d, uint64_t a, uint64_t b
         tc_mma_f16(tmem_d, a + at, b + at, idesc, kk > 0 ? 1u : 0u);
     }
 }
-// D[128 x head_dim] (+)= A B over 128 keys (rows), A in tensor memory as 16-bit pairs, B MN-major.
+// D[128 x head_dim] (+)= A B over half of a tile's keys, A in tensor memory as 16-bit pairs, B MN-major.  kPart 0: keys
+// 0-63, 1: keys 64-127.
+template <int kPart>
 __device__ __forceinline__ void mma_keys(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, bool accumulate) {
 #pragma unroll
-    for (int kk = 0; kk < kRowsTile / 16; ++kk)
-        tc_mma_f16_ts(tmem_d, tmem_a + (uint32_t)(8 * kk), b + (uint64_t)(kk * (2048 >> 4)), idesc, accumulate || kk > 0 ? 1u : 0u);
+    for (int i = 0; i < 4; ++i) {
+        const int kk = 4 * kPart + i;
+        tc_mma_f16_ts(tmem_d, tmem_a + (uint32_t)(8 * kk), b + (uint64_t)(kk * (2048 >> 4)), idesc, accumulate || i > 0 ? 1u : 0u);
+    }
 }
-
+__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, int* abort_flag, uint32_t* status) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status)) != 0;
+}
+__device__ __forceinline__ void arrive_warp(uint64_t* bar, int lane) {
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+}
 __device__ __forceinline__ void tc_st_32x32b_x32(uint32_t taddr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -98,6 +137,32 @@ __device__ __forceinline__ void tc_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]
 __device__ __forceinline__ void tc_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+
+__device__ __forceinline__ uint64_t f2_sub(uint64_t a, uint64_t b) { return f2_add(a, b ^ 0x8000000080000000ull); }
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// 2^x of two values on the FMA pipe: x = n + f, n the nearest integer (by adding 1.5 * 2^23, which leaves n in the low
+// bits), 2^f by its polynomial of degree 4 with the smallest largest relative error on [-1/2, 1/2] (2.6e-6, found by
+// Remez exchange), 2^n from the exponent bits.  x is kept above -125 (2^-125 in place of anything smaller); NaN stays.
+// The MUFU units give 16 exponentials a cycle and SM, this form takes a quarter of them off their hands.
+__device__ __forceinline__ void exp2_pair(uint64_t x, float& a, float& b) {
+    float x0, x1, t0, t1;
+    f2_unpack(x, x0, x1);
+    x = f2_pack(fmax_nan(x0, -125.0f), fmax_nan(x1, -125.0f));
+    const uint64_t magic = f2_pack(12582912.0f, 12582912.0f);
+    const uint64_t t = f2_add(x, magic);
+    const uint64_t f = f2_sub(x, f2_sub(t, magic));
+    uint64_t y = f2_fma(f2_pack(0.009570102207362652f, 0.009570102207362652f), f, f2_pack(0.05591785907745361f, 0.05591785907745361f));
+    y = f2_fma(y, f, f2_pack(0.240247443318367f, 0.240247443318367f));
+    y = f2_fma(y, f, f2_pack(0.6931217908859253f, 0.6931217908859253f));
+    y = f2_fma(y, f, f2_pack(0.9999992847442627f, 0.9999992847442627f));
+    f2_unpack(t, t0, t1);
+    const uint64_t scale = f2_pack(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u));
+    f2_unpack(f2_mul(y, scale), a, b);
 }
 
 // Zeroes rows [from, 128) of a tile in shared memory (all lanes of a warp), for the tensor cores to read: what TMA
@@ -125,10 +190,10 @@ __device__ __forceinline__ void store_row32(void* to, const uint32_t (&r)[32], f
     }
 }
 
-// Zero rows [from, to) of a contiguous 16-bit [rows, heads, head_dim] tensor, one head, by all threads of the CTA.
-__device__ __forceinline__ void zero_tail(void* base, int from, int to, int head, int heads, int dim) {
+// Zero rows [from, to) of a contiguous 16-bit [rows, heads, head_dim] tensor, one head, by thread `me` of `threads`.
+__device__ __forceinline__ void zero_tail(void* base, int from, int to, int head, int heads, int dim, int me, int threads) {
     const int chunks = dim / 8;
-    for (int i = threadIdx.x; i < (to - from) * chunks; i += blockDim.x) {
+    for (int i = me; i < (to - from) * chunks; i += threads) {
         const int row = from + i / chunks, c = i % chunks;
         reinterpret_cast<uint4*>(base)[((size_t)row * heads + head) * chunks + c] = make_uint4(0u, 0u, 0u, 0u);
     }

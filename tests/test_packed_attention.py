@@ -92,7 +92,7 @@ def _reference(q, k, v, do, lengths, scale, causal):
             # fp32: a score is off by (d + 8) steps of its sum of magnitudes, relative in the weight and again in the row's
             # sum; 2^-20 for the exponential; P rounded once to 16 bits (relative u; in fp16 also 2^-25 of 2^8 at most,
             # the running maximum being kept within 2^8)
-            off = 2 * (d + 8) * 2.0 ** -24 * ((qh.abs() @ kh.abs().T) * abs(scale) * seen).amax(-1, keepdim=True) + 2.0 ** -20
+            off = 2 * (d + 8) * 2.0 ** -24 * ((qh.abs() @ kh.abs().T) * abs(scale) * seen).amax(-1, keepdim=True) + 2.0 ** -18
             p_max = p.amax(-1, keepdim=True)
             floor = tiny * p_max                            # an unnormalised weight 1 stands for at least p_max / 2^8 .. p_max
             e_p = (u + off) * p + floor * seen              # error of the weights that multiply V, per element
