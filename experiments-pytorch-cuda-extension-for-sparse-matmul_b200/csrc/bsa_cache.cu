@@ -8,9 +8,11 @@
 //     infinity or a NaN gets a scale that is none either, so it never reads back as ordinary numbers.
 //     Reading gives round16(code * scale): one rounding to 16 bits, of the product held in fp32.
 //
-// One 16-byte chunk (8 elements) of a token's head per thread: head_dim / 8 neighbouring lanes hold one row, its maximum
-// is log2(head_dim / 8) shuffles, every load is 16 bytes and every store 8 (codes) or 16.  Both kernels move each byte
-// once: bound by DRAM at prompt sizes, by the launch at decoding sizes.
+// 16 elements of a token's head per thread: head_dim / 16 neighbouring lanes hold a row, whose maximum is that of packed
+// 16-bit magnitudes and two or three shuffles; a lane group takes one token and up to four of its heads, keys and values,
+// so a token's place is computed once and up to eight 32-byte loads are in flight.  Both kernels move each byte once:
+// bound by DRAM at prompt sizes, by the launch at decoding sizes.  (One row and side per lane group of 16 lanes spent
+// its time on addresses: 36 us for 16,000 tokens of 8 x 128.)
 #include <cuda_fp8.h>
 
 #include "bsa_common.cuh"
@@ -21,6 +23,9 @@ namespace {
 constexpr float kE4m3Max = 448.0f;
 constexpr float kAmaxFloor = 0x1p-100f;
 
+constexpr int kWideHeads = 2;
+constexpr int64_t kNarrowRows = 4096;          // tokens x heads below which a lane group takes one row
+
 struct CacheParams {
     const void* src[2];             // write: the tokens' keys / values; read: the cache's
     void* dst[2];
@@ -28,154 +33,174 @@ struct CacheParams {
     int64_t token_stride[2], head_stride[2];      // of the tokens' tensors, in elements
     const int64_t* slots;
     int64_t slot_count;             // pages * page
-    uint32_t rows, heads;           // rows = tokens * heads
-    int page_shift;
+    int tokens, heads, page_shift;
+    int wide[2];                    // the tokens' rows start on 32 bytes
     uint32_t* status;
 };
 
-template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
-    const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = Scalar<T>::to_float(e[i]);
+struct Words { uint32_t w[8]; };    // 16 elements of 16 bits
+
+__device__ __forceinline__ Words load_words(const void* p, bool wide) {
+    Words r;
+    if (wide) {
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7]) : "l"(p));
+    } else {
+        *reinterpret_cast<uint4*>(r.w) = static_cast<const uint4*>(p)[0];
+        *reinterpret_cast<uint4*>(r.w + 4) = static_cast<const uint4*>(p)[1];
+    }
+    return r;
+}
+__device__ __forceinline__ void store_words(void* p, const Words& r) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(p), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]), "r"(r.w[3]), "r"(r.w[4]), "r"(r.w[5]), "r"(r.w[6]), "r"(r.w[7]) : "memory");
 }
 
-__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-    return lo | (hi << 16);
-}
-
-// A slot behind the cache's end is reported and skipped like a negative one.
-__device__ __forceinline__ int64_t checked_slot(const CacheParams& p, uint32_t token) {
+// The slot of a token; one behind the cache's end is reported and skipped like a negative one.
+__device__ __forceinline__ int64_t checked_slot(const CacheParams& p, int token) {
     const int64_t slot = p.slots[token];
     if (slot < p.slot_count) return slot;
     atomicExch(p.status, (uint32_t)BSA_ERR_BAD_SHAPE);
     return -1;
 }
 
-// Row of the cache that holds `slot` of `head`.
-__device__ __forceinline__ int64_t cache_row(const CacheParams& p, int64_t slot, uint32_t head) {
-    return (((slot >> p.page_shift) * p.heads + head) << p.page_shift) + (slot & ((1 << p.page_shift) - 1));
-}
+template <typename T> __device__ __forceinline__ float2 unpack_word(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack_word<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <> __device__ __forceinline__ float2 unpack_word<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 
-// kRows: rows of a lane group, 1 where the grid is small (a decoding step), 4 at prompt sizes, so that four loads are in
-// flight per thread.
-template <typename T, bool kE4m3, int kDim, int kRows>
+// (an index that is not known when compiling would put the parameters into local memory)
+template <typename A>
+__device__ __forceinline__ A of(const A (&pair)[2], int side) { return side ? pair[1] : pair[0]; }
+
+// kHeads heads and kSides of keys and values per lane group: 1 and 1 (the side in blockIdx.z) where the grid is small.
+template <typename T, bool kE4m3, int kDim, int kHeads, int kSides>
 __global__ void __launch_bounds__(256) cache_write_kernel(const CacheParams p) {
-    constexpr int kLanes = kDim / 8;
-    constexpr uint32_t kStep = 256 / kLanes;
-    const int side = blockIdx.y, lane = threadIdx.x % kLanes;
-    const uint32_t first = blockIdx.x * (kRows * kStep) + threadIdx.x / kLanes;
-    uint4 w[kRows];
-    int64_t at[kRows];
+    constexpr int kLanes = kDim / 16, kTokens = 256 / kLanes;
+    const int lane = threadIdx.x % kLanes, token = blockIdx.x * kTokens + threadIdx.x / kLanes;
+    const int head0 = blockIdx.y * kHeads, heads = min(kHeads, p.heads - head0);
+    const int side0 = kSides == 2 ? 0 : blockIdx.z;
+    const int64_t slot = token < p.tokens ? checked_slot(p, token) : -1;
+    // row of the cache: page, head, place
+    const int64_t row = (((slot >> p.page_shift) * p.heads + head0) << p.page_shift) + (slot & ((1 << p.page_shift) - 1));
+    Words x[kHeads][kSides];
+    if (slot >= 0) {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        const uint32_t row = first + i * kStep;
-        at[i] = -1;
-        w[i] = make_uint4(0, 0, 0, 0);
-        if (row >= p.rows) continue;
-        const uint32_t token = row / p.heads, head = row - token * p.heads;
-        w[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.src[side]) + token * p.token_stride[side] +
-                                               head * p.head_stride[side] + lane * 8);
-        const int64_t slot = checked_slot(p, token);
-        if (slot >= 0) at[i] = cache_row(p, slot, head);
+        for (int i = 0; i < kSides; ++i) {
+            const int side = side0 + i;
+            const T* from = static_cast<const T*>(of(p.src, side)) + token * of(p.token_stride, side) + head0 * of(p.head_stride, side) + lane * 16;
+#pragma unroll
+            for (int h = 0; h < kHeads; ++h)
+                if (h < heads) x[h][i] = load_words(from + h * of(p.head_stride, side), of(p.wide, side) != 0);
+        }
+    }
+    if (!kE4m3) {
+        if (slot < 0) return;
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+            for (int i = 0; i < kSides; ++i)
+                if (h < heads) store_words(static_cast<T*>(of(p.dst, side0 + i)) + ((row + ((int64_t)h << p.page_shift)) * kDim + lane * 16), x[h][i]);
+        return;
     }
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        if (kE4m3) {
-            float x[8];
-            unpack8<T>(w[i], x);
+    for (int h = 0; h < kHeads; ++h) {
+        if (h >= heads) break;
+        const int64_t at = row + ((int64_t)h << p.page_shift);
+#pragma unroll
+        for (int i = 0; i < kSides; ++i) {
+            const int side = side0 + i;
+            const Words& v = x[h][i];
             // magnitudes compared as integers: the order of the bit patterns puts NaN above infinity, so neither is lost
-            uint32_t top = __float_as_uint(kAmaxFloor);
+            uint32_t top = v.w[0] & 0x7fff7fffu;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+            for (int e = 1; e < 8; ++e) top = __vmaxu2(top, v.w[e] & 0x7fff7fffu);
 #pragma unroll
-            for (int s = kLanes / 2; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, s));
-            const float amax = __uint_as_float(top), inv = __fdiv_rn(kE4m3Max, amax);
-            if (at[i] < 0) continue;
-            uint2 c;
-            c.x = codes4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-            c.y = codes4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
-            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.dst[side]) + at[i] * kDim + lane * 8) = c;
-            if (lane == 0) p.scales[side][at[i]] = __fdiv_rn(amax, kE4m3Max);
-        } else if (at[i] >= 0) {
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.dst[side]) + at[i] * kDim + lane * 8) = w[i];
-        }
-    }
-}
-
-__device__ __forceinline__ float2 values2(uint32_t codes) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3);
-    return __half22float2(*reinterpret_cast<const __half2*>(&h));
-}
-
-template <typename T, bool kE4m3, int kDim, int kRows>
-__global__ void __launch_bounds__(256) cache_read_kernel(const CacheParams p) {
-    constexpr int kLanes = kDim / 8;
-    constexpr uint32_t kStep = 256 / kLanes;
-    const int side = blockIdx.y, lane = threadIdx.x % kLanes;
-    const uint32_t first = blockIdx.x * (kRows * kStep) + threadIdx.x / kLanes;
-    int64_t at[kRows];
+            for (int s = kLanes / 2; s > 0; s >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, s));
+            const float2 both = unpack_word<T>(top);
+            const float amax = __uint_as_float(max(max(__float_as_uint(both.x), __float_as_uint(both.y)), __float_as_uint(kAmaxFloor)));
+            const float inv = __fdiv_rn(kE4m3Max, amax);
+            uint32_t codes[4];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        const uint32_t row = first + i * kStep;
-        at[i] = -1;
-        if (row >= p.rows) continue;
-        const uint32_t token = row / p.heads;
-        const int64_t slot = checked_slot(p, token);
-        if (slot >= 0) at[i] = cache_row(p, slot, row - token * p.heads);
-    }
-    uint4 w[kRows];
-    float scale[kRows];
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        w[i] = make_uint4(0, 0, 0, 0);
-        scale[i] = 0.0f;
-        if (at[i] < 0) continue;
-        if (kE4m3) {
-            const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.src[side]) + at[i] * kDim + lane * 8);
-            w[i].x = c.x; w[i].y = c.y;
-            scale[i] = p.scales[side][at[i]];
-        } else {
-            w[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.src[side]) + at[i] * kDim + lane * 8);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        const uint32_t row = first + i * kStep;
-        if (row >= p.rows) continue;
-        if (kE4m3) {
-            const uint32_t c[4] = {w[i].x & 0xffffu, w[i].x >> 16, w[i].y & 0xffffu, w[i].y >> 16};
-            uint4 out;
-            T* e = reinterpret_cast<T*>(&out);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const float2 v = values2(c[u]);
-                e[2 * u] = Scalar<T>::from_float(v.x * scale[i]);
-                e[2 * u + 1] = Scalar<T>::from_float(v.y * scale[i]);
+            for (int e = 0; e < 4; ++e) {
+                const float2 a = unpack_word<T>(v.w[2 * e]), b = unpack_word<T>(v.w[2 * e + 1]);
+                codes[e] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a.x * inv, a.y * inv), __NV_SATFINITE, __NV_E4M3) |
+                           (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(b.x * inv, b.y * inv), __NV_SATFINITE, __NV_E4M3) << 16;
             }
-            w[i] = out;
+            if (slot < 0) continue;
+            *reinterpret_cast<uint4*>(static_cast<uint8_t*>(of(p.dst, side)) + at * kDim + lane * 16) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+            if (lane == 0) of(p.scales, side)[at] = __fdiv_rn(amax, kE4m3Max);
         }
-        *reinterpret_cast<uint4*>(static_cast<T*>(p.dst[side]) + (size_t)row * kDim + lane * 8) = w[i];
     }
 }
 
+// Two codes (low 16 bits), scaled and rounded once to the 16-bit type.
+template <typename T>
+__device__ __forceinline__ uint32_t values2(uint32_t codes, float scale) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3);
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    T r[2] = {Scalar<T>::from_float(v.x * scale), Scalar<T>::from_float(v.y * scale)};
+    return *reinterpret_cast<const uint32_t*>(r);
+}
+
+template <typename T, bool kE4m3, int kDim, int kHeads, int kSides>
+__global__ void __launch_bounds__(256) cache_read_kernel(const CacheParams p) {
+    constexpr int kLanes = kDim / 16, kTokens = 256 / kLanes;
+    const int lane = threadIdx.x % kLanes, token = blockIdx.x * kTokens + threadIdx.x / kLanes;
+    if (token >= p.tokens) return;
+    const int head0 = blockIdx.y * kHeads, heads = min(kHeads, p.heads - head0);
+    const int side0 = kSides == 2 ? 0 : blockIdx.z;
+    const int64_t slot = checked_slot(p, token);
+    const int64_t row = (((slot >> p.page_shift) * p.heads + head0) << p.page_shift) + (slot & ((1 << p.page_shift) - 1));
+    Words x[kHeads][kSides];
+    float scale[kHeads][kSides];
+#pragma unroll
+    for (int i = 0; i < kSides; ++i)
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            const int side = side0 + i;
+            scale[h][i] = 0.0f;
+            x[h][i] = Words{};
+            if (h >= heads || slot < 0) continue;
+            const int64_t at = row + ((int64_t)h << p.page_shift);
+            if (kE4m3) {
+                *reinterpret_cast<uint4*>(x[h][i].w) = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(of(p.src, side)) + at * kDim + lane * 16);
+                scale[h][i] = of(p.scales, side)[at];
+            } else {
+                x[h][i] = load_words(static_cast<const T*>(of(p.src, side)) + at * kDim + lane * 16, true);
+            }
+        }
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+        for (int i = 0; i < kSides; ++i) {
+            if (h >= heads) continue;
+            Words v = x[h][i];
+            if (kE4m3) {
+#pragma unroll
+                for (int e = 3; e >= 0; --e) {
+                    const uint32_t c = v.w[e];
+                    v.w[2 * e] = values2<T>(c & 0xffffu, scale[h][i]);
+                    v.w[2 * e + 1] = values2<T>(c >> 16, scale[h][i]);
+                }
+            }
+            store_words(static_cast<T*>(of(p.dst, side0 + i)) + ((int64_t)token * p.heads + head0 + h) * kDim + lane * 16, v);
+        }
+}
+
+template <typename T, bool kE4m3, int kDim, int kHeads, int kSides>
+int launch_shape(bool write, const CacheParams& p, cudaStream_t stream) {
+    constexpr int kTokens = 256 / (kDim / 16);
+    const dim3 grid((unsigned)((p.tokens + kTokens - 1) / kTokens), (unsigned)((p.heads + kHeads - 1) / kHeads), 2 / kSides);
+    if (write) cache_write_kernel<T, kE4m3, kDim, kHeads, kSides><<<grid, 256, 0, stream>>>(p);
+    else cache_read_kernel<T, kE4m3, kDim, kHeads, kSides><<<grid, 256, 0, stream>>>(p);
+    return launch_status();
+}
 template <typename T, bool kE4m3, int kDim>
 int launch(bool write, const CacheParams& p, cudaStream_t stream) {
-    constexpr uint32_t kStep = 256 / (kDim / 8);
-    // 4 rows per lane group once even that grid fills the SMs (148 x 8 CTAs)
-    const bool wide = p.rows >= 2u * 1184u * kStep;
-    const uint32_t per_cta = kStep * (wide ? 4 : 1);
-    const dim3 grid((p.rows + per_cta - 1) / per_cta, 2);
-    if (write) {
-        if (wide) cache_write_kernel<T, kE4m3, kDim, 4><<<grid, 256, 0, stream>>>(p);
-        else cache_write_kernel<T, kE4m3, kDim, 1><<<grid, 256, 0, stream>>>(p);
-    } else {
-        if (wide) cache_read_kernel<T, kE4m3, kDim, 4><<<grid, 256, 0, stream>>>(p);
-        else cache_read_kernel<T, kE4m3, kDim, 1><<<grid, 256, 0, stream>>>(p);
-    }
-    return launch_status();
+    // few rows: one load per thread is the shortest way; many: eight in flight
+    const int64_t rows = (int64_t)p.tokens * p.heads;
+    return rows < kNarrowRows ? launch_shape<T, kE4m3, kDim, 1, 1>(write, p, stream)
+                              : launch_shape<T, kE4m3, kDim, kWideHeads, 2>(write, p, stream);
 }
 
 template <typename T>
@@ -194,15 +219,18 @@ int run_cache(bool write, int dtype, int store, CacheParams& p, int64_t tokens, 
     if (tokens == 0) return BSA_OK;
     for (int side = 0; side < 2; ++side) {
         if (!p.src[side] || !p.dst[side]) return BSA_ERR_NULL_POINTER;
-        if (!aligned16(p.src[side]) || !aligned16(p.dst[side])) return BSA_ERR_ALIGNMENT;
+        // the cache is read and written 32 bytes at a time, and so is the output of a read
+        if (!aligned16(p.src[side]) || (reinterpret_cast<uintptr_t>(p.dst[side]) & 31)) return BSA_ERR_ALIGNMENT;
+        if (!write && (reinterpret_cast<uintptr_t>(p.src[side]) & 31)) return BSA_ERR_ALIGNMENT;
         if (p.token_stride[side] < 0 || p.head_stride[side] < 0) return BSA_ERR_BAD_SHAPE;
         if (p.token_stride[side] % 8 != 0 || p.head_stride[side] % 8 != 0) return BSA_ERR_ALIGNMENT;
+        p.wide[side] = (reinterpret_cast<uintptr_t>(p.src[side]) & 31) == 0 && p.token_stride[side] % 16 == 0 && p.head_stride[side] % 16 == 0;
     }
     if (!p.slots) return BSA_ERR_NULL_POINTER;
-    if (tokens > (int64_t)INT32_MAX / (heads * (dim / 8))) return BSA_ERR_TOO_LARGE;       // 32-bit chunk numbers
+    if (tokens > (int64_t)INT32_MAX - 256) return BSA_ERR_TOO_LARGE;                        // 32-bit token numbers
     p.slot_count = pages * page;
-    p.rows = (uint32_t)(tokens * heads);
-    p.heads = (uint32_t)heads;
+    p.tokens = (int)tokens;
+    p.heads = (int)heads;
     p.page_shift = 0;
     while ((1 << p.page_shift) < page) ++p.page_shift;
     p.status = static_cast<uint32_t*>(workspace);

@@ -280,7 +280,8 @@ int bsa_packed_backward(int dtype, const void* q, int64_t q_token_stride, int64_
  *                   skipped and reported (BSA_ERR_BAD_SHAPE in the workspace).
  *                   The non-negative slots of one write must differ: two tokens
  *                   written to one slot leave a row mixed from both.
- *   keys, values    [pages, heads, page, head_dim], contiguous
+ *   keys, values    [pages, heads, page, head_dim], contiguous, 32-byte aligned, as
+ *                   the k and v that a read writes
  *   key_scales,
  *   value_scales    e4m3: float [pages, heads, page]; else ignored
  * page 16, 32, 64 or 128; head_dim 64 or 128; pages * heads * page < 2^31.

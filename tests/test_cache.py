@@ -27,9 +27,9 @@ def test_cache_validation_codes(lib):
     i, p = ctypes.c_int64, ctypes.c_void_p
     f.argtypes = [ctypes.c_int] * 2 + [p, p, i, i, i, i, p, i, p, p, p, p, i, i, i, i, p, ctypes.c_size_t, p]
 
-    def call(dtype=1, store=0, k=16, strides=(1024, 128, 1024, 128), slots=16, tokens=1, keys=16, scales=None, pages=4,
+    def call(dtype=1, store=0, k=16, strides=(1024, 128, 1024, 128), slots=16, tokens=1, keys=32, scales=None, pages=4,
              heads=8, page=64, dim=128, ws=16, ws_bytes=256):
-        return f(dtype, store, k, 16, *strides, slots, tokens, keys, 16, scales, scales, pages, heads, page, dim, ws,
+        return f(dtype, store, k, 16, *strides, slots, tokens, keys, 32, scales, scales, pages, heads, page, dim, ws,
                  ws_bytes, None)
 
     assert call(dtype=0) == 3                                   # float32 tokens
@@ -38,7 +38,7 @@ def test_cache_validation_codes(lib):
     assert call(page=48) == 5 and call(page=0) == 5 and call(page=256) == 5
     assert call(dim=80) == 4 and call(pages=0) == 4 and call(heads=0) == 4 and call(tokens=-1) == 4
     assert call(strides=(-1024, 128, 1024, 128)) == 4
-    assert call(strides=(1020, 128, 1024, 128)) == 6 and call(k=24) == 6 and call(keys=8) == 6
+    assert call(strides=(1020, 128, 1024, 128)) == 6 and call(k=24) == 6 and call(keys=16) == 6
     assert call(k=None) == 1 and call(slots=None) == 1
     assert call(ws=None) == 7 and call(ws_bytes=255) == 7
     assert call(pages=2 ** 31) == 10 and call(tokens=2 ** 31) == 10
