@@ -13,9 +13,9 @@
 // 8 x 128 x 128 x D operations, 1024 x D / 64 cycles of the tensor pipe at its peak, and 2 x 128 x 128 exponentials,
 // 2048 cycles of the four MUFU units: at D = 128 the two balance, at D = 64 the exponentials bind.
 //
-// The CTAs are persistent (one per SM, the items in a fixed order that alternates its direction, so that no SM gets the
-// longer one of every round): while the softmax warps end one item, the producer already loads the next one's Q and K and
-// its first scores are computed.
+// The CTAs are persistent (one per SM): a CTA takes over the places of CTAs of the grid that have not started (cluster
+// launch control), so the list of tiles, longest first, is shared out as SMs come free; while the softmax warps end one
+// item, the producer already loads the next one's Q and K and its first scores are computed.
 //   warps 0-3, 4-7   softmax of tile 0 / 1, one row per thread; the epilogue
 //   warp 8           TMA producer: items, Q, then K and V tiles through a ring of 4 stages
 //   warp 9           MMA issuer: S0 S1 | PV0 S0' PV1 S1' | ..; each PV in two parts, the first while the second half of P is made
@@ -46,14 +46,16 @@ struct __align__(16) FwdBarriers {
     uint64_t item_full[2], item_empty[2];
     uint64_t q_full[2], q_empty[2], full[kFwdStages], empty[kFwdStages];
     uint64_t s_full[2], p_full[2][2], o_full[2];
-    uint64_t drain;
+    uint64_t drain, stolen;
+    uint4 response;                             // of the request for another CTA's place
     int4 items[2];                              // first row of the sequence, its length, the tile, the first head; length 0: no more
     uint32_t tmem_base;
     int abort_flag;
 };
 
+constexpr int kStoreBytes = 8 * 32 * 128;       // a store stage per softmax warp
 template <int kDim>
-constexpr int fwd_smem() { return (2 + kFwdStages) * (kDim / 64) * kPanelBytes + (int)sizeof(FwdBarriers); }
+constexpr int fwd_smem() { return (2 + kFwdStages) * (kDim / 64) * kPanelBytes + kStoreBytes + (int)sizeof(FwdBarriers); }
 
 // What an item means: K / V tiles of each of its two Q tiles.
 struct FwdItem {
@@ -73,11 +75,13 @@ struct FwdItem {
 template <bool kBf16, int kDim>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap map_q,
-                      const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+                      const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                      const __grid_constant__ CUtensorMap map_o) {
     constexpr int kPanels = kDim / 64, kTile_ = kPanels * kPanelBytes;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* ring = smem + 2 * kTile_;
-    FwdBarriers* bars = reinterpret_cast<FwdBarriers*>(ring + kFwdStages * kTile_);
+    uint8_t* store_smem = ring + kFwdStages * kTile_;
+    FwdBarriers* bars = reinterpret_cast<FwdBarriers*>(store_smem + kStoreBytes);
     int* abort_flag = &bars->abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -96,6 +100,7 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
             mbar_init(&bars->p_full[i][0], 4); mbar_init(&bars->p_full[i][1], 4);
         }
         mbar_init(&bars->drain, 1);
+        mbar_init(&bars->stolen, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_shared();
     }
@@ -120,7 +125,7 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
     if (warp == 8) {
         // ------------------------------------------------------------ producer
         const int per_tile = p.pair ? kRowsTile : 2 * kRowsTile;
-        const int head_items = p.pair ? p.q_heads / 2 : p.q_heads, ctas = (int)gridDim.x;
+        const int head_items = p.pair ? p.q_heads / 2 : p.q_heads;
         int posted = 0, t = 0, q_no[2] = {0, 0};
         auto post = [&](const int4& v) {
             const int slot = posted & 1;
@@ -140,12 +145,35 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
             }
             __syncwarp();
         };
-        for (int round = 0; ok && (int64_t)round * ctas < p.items; ++round) {
-            const int64_t at = (int64_t)round * ctas + (round & 1 ? ctas - 1 - (int)blockIdx.x : (int)blockIdx.x);
-            if (at >= p.items) continue;
-            const int rank = (int)(at / head_items), head_item = (int)at - rank * head_items, head0 = p.pair ? 2 * head_item : head_item;
-            PackedItem found = packed_locate(p.offsets, p.batch, p.rows, per_tile, rank, lane, p.status);
-            if (found.length == 0) continue;
+        bool more = true, listed = true;
+        int at = (int)blockIdx.x, next = 0;
+        for (int round = 0; ok && more; ++round, at = next) {
+            // ask for the next item (the place of a CTA that has not started yet); the answer comes while this one's loads go out
+            if (lane == 0) {
+                mbar_expect_tx(&bars->stolen, 16);
+                asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                             ::"r"(smem_u32(&bars->response)), "r"(smem_u32(&bars->stolen)) : "memory");
+            }
+            __syncwarp();
+            auto take = [&]() {
+                if (!wait_all(&bars->stolen, (uint32_t)round & 1u, abort_flag, p.status)) { ok = false; return; }
+                uint32_t canceled;
+                asm volatile("{\n\t.reg .b128 r;\n\t.reg .pred c;\n\tld.shared.b128 r, [%2];\n\t"
+                             "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 c, r;\n\tselp.u32 %0, 1, 0, c;\n\t"
+                             "mov.u32 %1, 0;\n\t@c clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+                             : "=r"(canceled), "=r"(next) : "r"(smem_u32(&bars->response)) : "memory");
+                fence_async_shared();
+                __syncwarp();
+                more = canceled != 0;
+            };
+            const int rank = at / head_items, head_item = at - rank * head_items, head0 = p.pair ? 2 * head_item : head_item;
+            PackedItem found{0, 0, 0, 0};
+            if (listed) found = packed_locate(p.offsets, p.batch, p.rows, per_tile, rank, lane, p.status);
+            if (found.length == 0) {                            // behind the list's end, and so is everything after it
+                listed = false;
+                take();
+                continue;
+            }
             if (found.b == p.batch) {                           // rows behind the last sequence
                 const int from = found.start + found.tile * per_tile, to = min(from + per_tile, p.rows);
                 for (int h = head0; h <= head0 + p.pair; ++h) {
@@ -153,6 +181,7 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
                     if (p.lse)
                         for (int r = from + lane; r < to; r += 32) p.lse[(size_t)h * p.rows + r] = -INFINITY;
                 }
+                take();
                 continue;
             }
             const int4 v = make_int4(found.start, found.length, found.tile, head0);
@@ -171,6 +200,7 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
                 ok = wait_all(&bars->empty[stage], ((uint32_t)(t / kFwdStages) & 1u) ^ 1u, abort_flag, p.status);
                 if (ok) load(ring + stage * kTile_, j & 1 ? &map_v : &map_k, &bars->full[stage], kv_head, item.start + (j / 2) * kRowsTile);
             }
+            if (ok) take();
         }
         if (ok) post(make_int4(0, 0, 0, 0));
         if (lane == 0 && *(volatile int*)abort_flag) let_copies_land();
@@ -356,19 +386,27 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
             ok = wait_all(&bars->o_full[s], (uint32_t)o_no++ & 1u, abort_flag, p.status);
             if (!ok) break;
             tc_fence_after();
-            uint32_t acc[kDim / 32][32];
-#pragma unroll
-            for (int i = 0; i < kDim / 32; ++i) tc_ld_32x32b_x32(o_tmem + (uint32_t)(32 * i), acc[i]);
-            tc_wait_ld();
             const int head = p.pair ? item.head0 + s : item.head0;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            if (row < item.length) {
-                uint8_t* to = static_cast<uint8_t*>(p.o) + (((size_t)(item.start + row) * p.q_heads + head) * kDim) * 2;
+            const bool full = row - lane + 32 <= item.length;                       // all 32 rows of the warp
+            uint8_t* to = static_cast<uint8_t*>(p.o) + (((size_t)(item.start + row) * p.q_heads + head) * kDim) * 2;
 #pragma unroll
-                for (int i = 0; i < kDim / 32; ++i) store_row32<kBf16>(to + 64 * i, acc[i], inv);
-                if (p.lse) p.lse[(size_t)head * p.rows + item.start + row] = m + __log2f(l);
+            for (int i = 0; i < kDim / 64; ++i) {
+                uint32_t acc[2][32];
+                tc_ld_32x32b_x32(o_tmem + (uint32_t)(64 * i), acc[0]);
+                tc_ld_32x32b_x32(o_tmem + (uint32_t)(64 * i + 32), acc[1]);
+                tc_wait_ld();
+                if (full) {
+                    store_rows64<kBf16>(store_smem + warp * 4096, &map_o, acc, inv, 64 * i, head, item.start + row - lane, lane);
+                } else if (row < item.length) {
+                    store_row32<kBf16>(to + 128 * i, acc[0], inv);
+                    store_row32<kBf16>(to + 128 * i + 64, acc[1], inv);
+                }
             }
+            if (p.lse && row < item.length) p.lse[(size_t)head * p.rows + item.start + row] = m + __log2f(l);
         }
+        if (lane == 0) store_done();
+        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
@@ -380,16 +418,15 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
 }
 
 template <bool kBf16, int kDim>
-int launch_forward(PackedParams p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
+int launch_forward(PackedParams p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mo,
+                   cudaStream_t stream) {
     auto kernel = packed_forward_kernel<kBf16, kDim>;
     constexpr int smem = fwd_smem<kDim>();
     if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return BSA_ERR_LAUNCH;
     // an upper bound of the tiles: every sequence and the rows behind the last one may end inside a tile
     const int per_tile = p.pair ? kRowsTile : 2 * kRowsTile;
     p.items = (p.rows / per_tile + p.batch + 1) * (p.pair ? p.q_heads / 2 : p.q_heads);
-    const int sms = sm_count();
-    if (sms <= 0) return BSA_ERR_LAUNCH;
-    kernel<<<p.items < sms ? p.items : sms, kFwdThreads, smem, stream>>>(p, mq, mk, mv);
+    kernel<<<p.items, kFwdThreads, smem, stream>>>(p, mq, mk, mv, mo);
     return launch_status();
 }
 
@@ -419,13 +456,14 @@ extern "C" int bsa_packed_forward(int dtype, const void* q, int64_t q_token_stri
     // a scale of 0 stays a factor that keeps masked scores at -infinity
     p.scale_log2 = fmaxf(fabsf(scale) * kPackedLog2e, 1e-37f);
     p.status = static_cast<uint32_t*>(workspace);
-    CUtensorMap mq, mk, mv;
+    CUtensorMap mq, mk, mv, mo;
     if (!bind_device()) return BSA_ERR_LAUNCH;
     if (!make_packed_map(&mq, dtype, q, rows, q_heads, head_dim, q_token_stride, q_head_stride) ||
         !make_packed_map(&mk, dtype, k, rows, kv_heads, head_dim, k_token_stride, k_head_stride) ||
-        !make_packed_map(&mv, dtype, v, rows, kv_heads, head_dim, v_token_stride, v_head_stride)) return BSA_ERR_DRIVER;
+        !make_packed_map(&mv, dtype, v, rows, kv_heads, head_dim, v_token_stride, v_head_stride) ||
+        !make_packed_map(&mo, dtype, o, rows, q_heads, head_dim, q_heads * head_dim, head_dim, 32)) return BSA_ERR_DRIVER;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == BSA_DTYPE_BF16)
-        return head_dim == 64 ? launch_forward<true, 64>(p, mq, mk, mv, s) : launch_forward<true, 128>(p, mq, mk, mv, s);
-    return head_dim == 64 ? launch_forward<false, 64>(p, mq, mk, mv, s) : launch_forward<false, 128>(p, mq, mk, mv, s);
+        return head_dim == 64 ? launch_forward<true, 64>(p, mq, mk, mv, mo, s) : launch_forward<true, 128>(p, mq, mk, mv, mo, s);
+    return head_dim == 64 ? launch_forward<false, 64>(p, mq, mk, mv, mo, s) : launch_forward<false, 128>(p, mq, mk, mv, mo, s);
 }

@@ -208,6 +208,30 @@ __device__ __forceinline__ void store_row32(void* to, const uint32_t (&r)[32], f
     }
 }
 
+// Rows of a warp to global memory, 64 columns at a time: through shared memory (`stage`: 32 rows x 128 bytes of this warp,
+// swizzled) and a TMA store where all 32 rows belong to the sequence, else row by row.  (A row per thread stored straight
+// from registers touches 32 lines per instruction: an epilogue of 128 x 128 took 3000-4000 cycles.)
+__device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+template <bool kBf16>
+__device__ __forceinline__ void store_rows64(uint8_t* stage, const CUtensorMap* map, const uint32_t (&r)[2][32], float by, int column,
+                                             int head, int row, int lane) {
+    if (lane == 0) store_done();                // the last store has read the stage
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            w[e] = pack2<kBf16>(__uint_as_float(r[u / 4][8 * (u % 4) + 2 * e]) * by, __uint_as_float(r[u / 4][8 * (u % 4) + 2 * e + 1]) * by);
+        *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    fence_async_shared();
+    __syncwarp();
+    if (lane == 0)
+        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];\n\tcp.async.bulk.commit_group;"
+                     ::"l"(map), "r"(smem_u32(stage)), "r"(column), "r"(head), "r"(row) : "memory");
+}
+
 // Zero rows [from, to) of a contiguous 16-bit [rows, heads, head_dim] tensor, one head, by thread `me` of `threads`.
 __device__ __forceinline__ void zero_tail(void* base, int from, int to, int head, int heads, int dim, int me, int threads) {
     const int chunks = dim / 8;
@@ -217,15 +241,15 @@ __device__ __forceinline__ void zero_tail(void* base, int from, int to, int head
     }
 }
 
-// Tensor map over [tokens, heads, head_dim] (16 bits, strides in elements): boxes of 64 elements x 1 head x 128 tokens.
+// Tensor map over [tokens, heads, head_dim] (16 bits, strides in elements): boxes of 64 elements x 1 head x box_rows tokens.
 // Rows behind the last read as zero.
 bool make_packed_map(CUtensorMap* map, int dtype, const void* base, int64_t tokens, int64_t heads, int64_t dim,
-                     int64_t token_stride, int64_t head_stride) {
+                     int64_t token_stride, int64_t head_stride, int box_rows = kRowsTile) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
     const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens};
     const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
-    const cuuint32_t box[3] = {64, 1, kRowsTile};
+    const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows};
     const cuuint32_t elem[3] = {1, 1, 1};
     const CUtensorMapDataType type = dtype == BSA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     return fn(map, type, 3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
