@@ -148,14 +148,15 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
         bool more = true, listed = true;
         int at = (int)blockIdx.x, next = 0;
         for (int round = 0; ok && more; ++round, at = next) {
-            // ask for the next item (the place of a CTA that has not started yet); the answer comes while this one's loads go out
-            if (lane == 0) {
-                mbar_expect_tx(&bars->stolen, 16);
-                asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
-                             ::"r"(smem_u32(&bars->response)), "r"(smem_u32(&bars->stolen)) : "memory");
-            }
-            __syncwarp();
+            // The next item: the place of a CTA that has not started yet.  Asked for once this one's loads are out, about two
+            // steps before its end: earlier, an SM with a long item would hold back another one.
             auto take = [&]() {
+                if (lane == 0) {
+                    mbar_expect_tx(&bars->stolen, 16);
+                    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                                 ::"r"(smem_u32(&bars->response)), "r"(smem_u32(&bars->stolen)) : "memory");
+                }
+                __syncwarp();
                 if (!wait_all(&bars->stolen, (uint32_t)round & 1u, abort_flag, p.status)) { ok = false; return; }
                 uint32_t canceled;
                 asm volatile("{\n\t.reg .b128 r;\n\t.reg .pred c;\n\tld.shared.b128 r, [%2];\n\t"
