@@ -173,7 +173,8 @@ struct CachedShape {
     static constexpr int kJoinFloats = kGroups == 4 ? 0 : kConsumers * 16 * (kJoin + 2);
     static constexpr int kRows = 16 * kGroups;
     static constexpr int kQueryBytes = kRows * (kDim * 2 + 4);                  // fragments, and a factor per row
-    static constexpr int kSmem = kStages * (kStageBytes + kScaleBytes) + kQueryBytes + kJoinFloats * 4 + (int)sizeof(CachedBarriers<kStages>);
+    static constexpr int kKeyBytes = kE4m3 ? kConsumers * 32 * 16 : 0;          // what the warps make of their keys' scales
+    static constexpr int kSmem = kStages * (kStageBytes + kScaleBytes) + kKeyBytes + kQueryBytes + kJoinFloats * 4 + (int)sizeof(CachedBarriers<kStages>);
     static_assert(2 * (kSmem + 1024) <= 233472, "two CTAs per SM");
 };
 
@@ -199,11 +200,12 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
     // too few independent instructions between the tile's barriers.
     constexpr int kStreams = kSplit == 4 ? 2 : 1;
     constexpr int kWarpKeys = kTileKeys * kStreams / kSplit;            // keys of a tile per warp
-    constexpr int kStepKeys = kWarpKeys < 32 ? kWarpKeys : 32;          // keys of a step of the warp (registers)
+    constexpr int kStepKeys = 32;                           // keys of a step of the warp (registers)
     constexpr int kNT = kStepKeys / 8;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* scale_smem = smem + S::kStages * S::kStageBytes;
-    uint32_t* q_smem = reinterpret_cast<uint32_t*>(scale_smem + S::kStages * S::kScaleBytes);     // [row group][k step][lane][4]
+    float4* key_smem = reinterpret_cast<float4*>(scale_smem + S::kStages * S::kScaleBytes);
+    uint32_t* q_smem = reinterpret_cast<uint32_t*>(scale_smem + S::kStages * S::kScaleBytes + S::kKeyBytes);     // [row group][k step][lane][4]
     float* q_factor = reinterpret_cast<float*>(q_smem + kRows * kDim / 2);
     float* merge = q_factor + kRows;
     Bars* bars = reinterpret_cast<Bars*>(merge + S::kJoinFloats);
@@ -428,20 +430,25 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
                     }
                 }
             }
-            // scores in units of log2; for e4m3 with the value's scale in the weight
-            const float* scales = reinterpret_cast<const float*>(scale_smem + stage * S::kScaleBytes) + base + 2 * c;
+            // scores in units of log2; for e4m3 with the value's scale in the weight.  A lane makes what a key needs of its
+            // scales, the warp shares it: (key's scale, log2 of the value's, 1 / the value's).
             float inv[kNT][2];
+            if (kE4m3) {
+                const float* scales = reinterpret_cast<const float*>(scale_smem + stage * S::kScaleBytes) + base + lane;
+                const float sv = scales[kTileKeys];
+                __syncwarp();                               // the last step's have been read
+                key_smem[warp * 32 + lane] = make_float4(scales[0], __log2f(sv), __fdividef(1.0f, sv), 0.0f);
+                __syncwarp();
+            }
 #pragma unroll
             for (int n = 0; n < kNT; ++n) {
                 if (kE4m3) {
-                    const float2 sk = *reinterpret_cast<const float2*>(scales + n * 8);
-                    const float2 sv = *reinterpret_cast<const float2*>(scales + kTileKeys + n * 8);
-                    const float lv[2] = {__log2f(sv.x), __log2f(sv.y)};
-                    inv[n][0] = __frcp_rn(sv.x);
-                    inv[n][1] = __frcp_rn(sv.y);
+                    const float4 k0 = key_smem[warp * 32 + n * 8 + 2 * c], k1 = key_smem[warp * 32 + n * 8 + 2 * c + 1];
+                    inv[n][0] = k0.z;
+                    inv[n][1] = k1.z;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        s[n][e] = fmaf(s[n][e] * ((e & 1) ? sk.y : sk.x), row_scale[e >> 1], lv[e & 1]);
+                        s[n][e] = fmaf(s[n][e] * ((e & 1) ? k1.x : k0.x), row_scale[e >> 1], (e & 1) ? k1.y : k0.y);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[n][e] *= row_scale[e >> 1];
