@@ -52,7 +52,6 @@ struct CachedParams {
     int batch, drafts, group, kv_heads, row_tiles, table_width, pages, page_shift;
     float scale_log2;                           // scale * log2 e
     float* partial;                             // [ctas][2][rows][head_dim], then [ctas][2][rows][2] of (m, l)
-    int2* parts;                                // [batch][kv_heads * row_tiles]: first and last CTA of each
     int ctas;
     uint32_t* status;
 };
@@ -77,13 +76,21 @@ __device__ __forceinline__ int cached_tiles(const CachedParams& p, int b) {
     return max(1, (cached_length(p, b) + kTileKeys - 1) / kTileKeys);
 }
 
-// Units of one head and row tile of the whole batch, by one warp.
-__device__ __forceinline__ int64_t total_cost(const CachedParams& p, int lane) {
-    int64_t sum = 0;
+// Units of one head and row tile of the whole batch, and of the sequences before `part` (in `before`), by one warp.
+__device__ __forceinline__ int64_t total_cost(const CachedParams& p, int part, int64_t& before, int lane) {
+    int64_t sum = 0, some = 0;
 #pragma unroll 4
-    for (int b = lane; b < p.batch; b += 32) sum += cached_tiles(p, b) + kBegin;
+    for (int b = lane; b < p.batch; b += 32) {
+        const int cost = cached_tiles(p, b) + kBegin;
+        sum += cost;
+        if (b < part) some += cost;
+    }
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    for (int s = 16; s > 0; s >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        some += __shfl_xor_sync(0xffffffffu, some, s);
+    }
+    before = some;
     return sum;
 }
 // a / b; the units fit 32 bits unless a batch holds more keys than the device's memory
@@ -96,7 +103,13 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 __device__ __forceinline__ Share find_share(const CachedParams& p, int cta, int lane) {
     Share s;
     const int hms = p.kv_heads * p.row_tiles;
-    const int64_t units = total_cost(p, lane) * hms;
+    // (the first 32 sequences stay in registers: with no more than those there is one load on the way to the first tile)
+    const int first = lane < p.batch ? cached_tiles(p, lane) + kBegin : 0;
+    int64_t sum = first;
+    for (int b = 32 + lane; b < p.batch; b += 32) sum += cached_tiles(p, b) + kBegin;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const int64_t units = sum * hms;
     s.per = quotient(units + p.ctas - 1, p.ctas);
     s.first = min((int64_t)cta * s.per, units);
     s.end = min(s.first + s.per, units);
@@ -104,7 +117,7 @@ __device__ __forceinline__ Share find_share(const CachedParams& p, int cta, int 
     if (s.first >= s.end) return s;
     int64_t before = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
-        const int mine = b0 + lane < p.batch ? cached_tiles(p, b0 + lane) + kBegin : 0;
+        const int mine = b0 == 0 ? first : (b0 + lane < p.batch ? cached_tiles(p, b0 + lane) + kBegin : 0);
         int64_t upto = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -127,11 +140,6 @@ __device__ __forceinline__ Share find_share(const CachedParams& p, int cta, int 
         before += __shfl_sync(0xffffffffu, upto, 31);
     }
     return s;
-}
-
-// How many CTAs after this one hold tiles of an item whose last unit is `last` (from the share's nominal end on).
-__device__ __forceinline__ int later_parts(int64_t last, const Share& s) {
-    return last < s.end ? 0 : 1 + (int)((uint32_t)min(last - s.end, (int64_t)UINT32_MAX) / (uint32_t)s.per);
 }
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
@@ -565,8 +573,6 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
         }
-        if (from_start && threadIdx.x == 0)
-            p.parts[(int64_t)b * hms + hm] = make_int2((int)blockIdx.x, (int)blockIdx.x + later_parts(u + tiles - 1, share));
         const int b_now = b, hm_now = hm;
         const bool on_now[2] = {row_on[0], row_on[1]};
         u += todo;
@@ -679,33 +685,48 @@ cached_join_kernel(const CachedParams p, int rows) {
     const int in_tile = rows / 4, item = blockIdx.x / in_tile, r = (blockIdx.x - item * in_tile) * 4 + warp;
     const int b = item / hms, hm = item - b * hms;
     const int head = hm / p.row_tiles, row = (hm - head * p.row_tiles) * rows + r, draft = row / p.group;
-    if (draft >= p.drafts) return;
+    // which CTAs hold this item's tiles follows from the lengths alone: found while the main kernel still runs
+    int64_t before;
+    const int64_t per = quotient(total_cost(p, b, before, lane) * hms + p.ctas - 1, p.ctas);
+    const int tiles = cached_tiles(p, b);
+    const int64_t start = before * hms + (int64_t)hm * (tiles + kBegin) + kBegin;       // the unit of tile 0
+    const int first = (int)quotient(start, per), last = (int)quotient(start + tiles - 1, per);
+    // (also where there is nothing to do: the stream's next kernel waits for this grid, which must not end before the main one)
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int2 parts = p.parts[item];
-    const int first = parts.x, last = parts.y;
-    if (first == last) return;                              // one CTA had all of it and wrote the output
+    if (draft >= p.drafts || first == last) return;         // one CTA had all of it and wrote the output
     const float* ml = p.partial + (int64_t)p.ctas * 2 * rows * kDim;
-    constexpr int kCols = kDim / 32;
-    float top = -INFINITY;
-    for (int i = first + lane; i <= last; i += 32) top = fmaxf(top, ml[(((int64_t)i * 2 + (i == first)) * rows + r) * 2]);
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float sum[kCols], l = 0.0f;
+    constexpr int kCols = kDim / 32, kBatch = 8;
+    float sum[kCols], l = 0.0f, top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < kCols; ++e) sum[e] = 0.0f;
-#pragma unroll 8
-    for (int i = first; i <= last; ++i) {                   // (slot 1: the CTA that has tile 0; slot 0: the ones after it)
-        const int64_t at = ((int64_t)i * 2 + (i == first)) * rows + r;
-        const float2 w = *reinterpret_cast<const float2*>(ml + at * 2);
-        const float* x = p.partial + at * kDim + lane * kCols;      // (zeros where this part saw nothing)
-        float v[kCols];
+    for (int i0 = first; i0 <= last; i0 += kBatch) {        // loads of 8 parts at a time, in the order of the tiles
+        float2 w[kBatch];
+        float v[kBatch][kCols];
 #pragma unroll
-        for (int e = 0; e < kCols; e += 2) *reinterpret_cast<float2*>(v + e) = *reinterpret_cast<const float2*>(x + e);
-        const float weight = attn_exp2(w.x - ref);
-        l += w.y * weight;
+        for (int k = 0; k < kBatch; ++k) {                  // (slot 1: the CTA that has tile 0; slot 0: the ones after it)
+            const int i = min(i0 + k, last);
+            const int64_t at = ((int64_t)i * 2 + (i == first)) * rows + r;
+            w[k] = *reinterpret_cast<const float2*>(ml + at * 2);
+            if (i0 + k > last) w[k] = make_float2(-INFINITY, 0.0f);
+            const float* x = p.partial + at * kDim + lane * kCols;      // (zeros where this part saw nothing)
 #pragma unroll
-        for (int e = 0; e < kCols; ++e) sum[e] += v[e] * weight;
+            for (int e = 0; e < kCols; e += 2) *reinterpret_cast<float2*>(v[k] + e) = *reinterpret_cast<const float2*>(x + e);
+        }
+        float higher = top;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) higher = fmaxf(higher, w[k].x);
+        const float ref = higher == -INFINITY ? 0.0f : higher, fall = attn_exp2(top - ref);
+        top = higher;
+        l *= fall;
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) sum[e] *= fall;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const float weight = attn_exp2(w[k].x - ref);
+            l += w[k].y * weight;
+#pragma unroll
+            for (int e = 0; e < kCols; ++e) sum[e] += v[k][e] * weight;
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T* to = static_cast<T*>(p.o) + (((int64_t)b * p.drafts + draft) * (p.kv_heads * p.group) + head * p.group + (row - draft * p.group)) * kDim + lane * kCols;
@@ -769,11 +790,10 @@ int launch_cached_typed(int store, int64_t dim, int groups, const CachedParams& 
 }  // namespace
 }  // namespace bsa
 
-extern "C" size_t bsa_cached_attention_scratch(int64_t batch, int64_t drafts, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
-    if (batch <= 0 || drafts <= 0 || kv_heads <= 0 || q_heads < kv_heads || head_dim <= 0) return 0;
+extern "C" size_t bsa_cached_attention_scratch(int64_t drafts, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
+    if (drafts <= 0 || kv_heads <= 0 || q_heads < kv_heads || head_dim <= 0) return 0;
     const int64_t rows = drafts * (q_heads / kv_heads), tile = 16 * bsa::row_groups(rows);
-    const size_t parts = (size_t)batch * kv_heads * ((rows + tile - 1) / tile) * sizeof(int2);
-    return parts + (size_t)std::max(bsa::sm_count(), 1) * 2 * 2 * tile * (size_t)(head_dim + 2) * 4;
+    return (size_t)std::max(bsa::sm_count(), 1) * 2 * 2 * tile * (size_t)(head_dim + 2) * 4;
 }
 
 extern "C" int bsa_cached_attention(int dtype, int store, const void* q, int64_t q_batch_stride, int64_t q_draft_stride,
@@ -819,8 +839,7 @@ extern "C" int bsa_cached_attention(int dtype, int store, const void* q, int64_t
     p.ctas = 2 * sm_count();
     p.status = static_cast<uint32_t*>(workspace);
     if (p.ctas <= 0) return BSA_ERR_LAUNCH;
-    p.parts = reinterpret_cast<int2*>(p.partial + (int64_t)p.ctas * 2 * 16 * groups * (head_dim + 2));
-    if (scratch_bytes < bsa_cached_attention_scratch(batch, drafts, q_heads, kv_heads, head_dim)) return BSA_ERR_WORKSPACE;
+    if (scratch_bytes < bsa_cached_attention_scratch(drafts, q_heads, kv_heads, head_dim)) return BSA_ERR_WORKSPACE;
     // the driver's encoder needs the device's context bound to this thread
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) { cudaGetLastError(); return BSA_ERR_LAUNCH; }

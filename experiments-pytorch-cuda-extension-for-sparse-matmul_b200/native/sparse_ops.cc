@@ -519,7 +519,7 @@ torch::Tensor cached_attention(torch::Tensor q, torch::Tensor keys, torch::Tenso
     if (batch == 0) return o;
     q = row_aligned(q);
     auto ws = workspace_for(q.device());
-    const size_t bytes = bsa_cached_attention_scratch(batch, drafts, heads, c.heads, c.dim);
+    const size_t bytes = bsa_cached_attention_scratch(drafts, heads, c.heads, c.dim);
     auto scratch = torch::empty({static_cast<int64_t>(bytes)}, q.options().dtype(torch::kUInt8));
     check_status(bsa_cached_attention(
         c.dtype, c.store, q.data_ptr(), axis_stride(q, 0), axis_stride(q, 1), axis_stride(q, 2), keys.data_ptr(),

@@ -326,8 +326,7 @@ int bsa_cache_read(int dtype, int store, const int64_t* slots, int64_t tokens, c
  *                   call alone until it is done
  * drafts <= 64.
  */
-size_t bsa_cached_attention_scratch(int64_t batch, int64_t drafts, int64_t q_heads, int64_t kv_heads,
-                                    int64_t head_dim);
+size_t bsa_cached_attention_scratch(int64_t drafts, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
 int bsa_cached_attention(int dtype, int store, const void* q, int64_t q_batch_stride, int64_t q_draft_stride,
                          int64_t q_head_stride, const void* keys, const void* values, const float* key_scales,
                          const float* value_scales, void* o, const int32_t* table, const int32_t* lengths,
