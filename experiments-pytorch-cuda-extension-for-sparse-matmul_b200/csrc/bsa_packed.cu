@@ -21,6 +21,8 @@
 //   warp 9           MMA issuer: S0 S1 | PV0 S0' PV1 S1' | ..; each PV in two parts, the first while the second half of P is made
 // The last K / V tile of a sequence may hold rows of the next one; its V rows are zeroed before use (see zero_rows).
 // All waits are bounded.
+#include <type_traits>
+
 #include "bsa_packed_common.cuh"
 
 namespace bsa {
@@ -32,7 +34,8 @@ constexpr int kPoly = 0;                        // every kPoly-th pair of expone
 
 struct PackedParams {
     void* o;
-    float* lse;                                 // [q_heads, rows], in units of log2, scale included; may be null
+    void* o_low;                                // what rounding took from o, in o's type
+    float* lse;                                 // [q_heads, rows], in units of log2, scale included
     const int32_t* offsets;
     int batch, rows, q_heads, kv_heads, group, causal;
     int items;                                  // upper bound of the work items
@@ -72,11 +75,12 @@ struct FwdItem {
     }
 };
 
-template <bool kBf16, int kDim>
+// kKeep: what a backward needs is kept (the rest of o, lse).
+template <bool kBf16, int kDim, bool kKeep>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap map_q,
                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                      const __grid_constant__ CUtensorMap map_o) {
+                      const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_low) {
     constexpr int kPanels = kDim / 64, kTile_ = kPanels * kPanelBytes;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* ring = smem + 2 * kTile_;
@@ -179,7 +183,8 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
                 const int from = found.start + found.tile * per_tile, to = min(from + per_tile, p.rows);
                 for (int h = head0; h <= head0 + p.pair; ++h) {
                     zero_tail(p.o, from, to, h, p.q_heads, kDim, lane, 32);
-                    if (p.lse)
+                    if (kKeep) zero_tail(p.o_low, from, to, h, p.q_heads, kDim, lane, 32);
+                    if (kKeep)
                         for (int r = from + lane; r < to; r += 32) p.lse[(size_t)h * p.rows + r] = -INFINITY;
                 }
                 take();
@@ -390,21 +395,33 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
             const int head = p.pair ? item.head0 + s : item.head0;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const bool full = row - lane + 32 <= item.length;                       // all 32 rows of the warp
-            uint8_t* to = static_cast<uint8_t*>(p.o) + (((size_t)(item.start + row) * p.q_heads + head) * kDim) * 2;
+            const size_t at = ((size_t)(item.start + row) * p.q_heads + head) * kDim;
+            uint8_t* stage = store_smem + warp * 4096;
 #pragma unroll
             for (int i = 0; i < kDim / 64; ++i) {
-                uint32_t acc[2][32];
+                uint32_t acc[2][32], w[32];
                 tc_ld_32x32b_x32(o_tmem + (uint32_t)(64 * i), acc[0]);
                 tc_ld_32x32b_x32(o_tmem + (uint32_t)(64 * i + 32), acc[1]);
                 tc_wait_ld();
-                if (full) {
-                    store_rows64<kBf16>(store_smem + warp * 4096, &map_o, acc, inv, 64 * i, head, item.start + row - lane, lane);
-                } else if (row < item.length) {
-                    store_row32<kBf16>(to + 128 * i, acc[0], inv);
-                    store_row32<kBf16>(to + 128 * i + 64, acc[1], inv);
+#pragma unroll
+                for (int e = 0; e < 64; e += 2) {
+                    acc[e / 32][e % 32] = __float_as_uint(__uint_as_float(acc[e / 32][e % 32]) * inv);
+                    acc[e / 32][e % 32 + 1] = __float_as_uint(__uint_as_float(acc[e / 32][e % 32 + 1]) * inv);
+                    w[e / 2] = pack2<kBf16>(__uint_as_float(acc[e / 32][e % 32]), __uint_as_float(acc[e / 32][e % 32 + 1]));
+                }
+                if (full) store_rows64(stage, &map_o, w, 64 * i, head, item.start + row - lane, lane);
+                else if (row < item.length) store_row64(static_cast<uint8_t*>(p.o) + (at + 64 * i) * 2, w);
+                if (kKeep) {
+#pragma unroll
+                    for (int e = 0; e < 64; e += 2) {
+                        const float2 v = word_values<kBf16>(w[e / 2]);
+                        w[e / 2] = pack2<kBf16>(__uint_as_float(acc[e / 32][e % 32]) - v.x, __uint_as_float(acc[e / 32][e % 32 + 1]) - v.y);
+                    }
+                    if (full) store_rows64(stage, &map_low, w, 64 * i, head, item.start + row - lane, lane);
+                    else if (row < item.length) store_row64(static_cast<uint8_t*>(p.o_low) + (at + 64 * i) * 2, w);
                 }
             }
-            if (p.lse && row < item.length) p.lse[(size_t)head * p.rows + item.start + row] = m + __log2f(l);
+            if (kKeep && row < item.length) p.lse[(size_t)head * p.rows + item.start + row] = m + __log2f(l);
         }
         if (lane == 0) store_done();
         __syncwarp();
@@ -418,16 +435,16 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
     }
 }
 
-template <bool kBf16, int kDim>
+template <bool kBf16, int kDim, bool kKeep>
 int launch_forward(PackedParams p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mo,
-                   cudaStream_t stream) {
-    auto kernel = packed_forward_kernel<kBf16, kDim>;
+                   const CUtensorMap& ml, cudaStream_t stream) {
+    auto kernel = packed_forward_kernel<kBf16, kDim, kKeep>;
     constexpr int smem = fwd_smem<kDim>();
     if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return BSA_ERR_LAUNCH;
     // an upper bound of the tiles: every sequence and the rows behind the last one may end inside a tile
     const int per_tile = p.pair ? kRowsTile : 2 * kRowsTile;
     p.items = (p.rows / per_tile + p.batch + 1) * (p.pair ? p.q_heads / 2 : p.q_heads);
-    kernel<<<p.items, kFwdThreads, smem, stream>>>(p, mq, mk, mv, mo);
+    kernel<<<p.items, kFwdThreads, smem, stream>>>(p, mq, mk, mv, mo, ml);
     return launch_status();
 }
 
@@ -436,7 +453,7 @@ int launch_forward(PackedParams p, const CUtensorMap& mq, const CUtensorMap& mk,
 
 extern "C" int bsa_packed_forward(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                                   int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
-                                  int64_t v_head_stride, void* o, float* lse, const int32_t* offsets, int64_t rows,
+                                  int64_t v_head_stride, void* o, void* o_low, float* lse, const int32_t* offsets, int64_t rows,
                                   int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scale, int causal,
                                   void* workspace, size_t workspace_bytes, void* stream) {
     using namespace bsa;
@@ -444,12 +461,12 @@ extern "C" int bsa_packed_forward(int dtype, const void* q, int64_t q_token_stri
     if (checked != BSA_OK) return checked;
     if (!workspace || workspace_bytes < BSA_WORKSPACE_BYTES) return BSA_ERR_WORKSPACE;
     if (rows == 0) return BSA_OK;
-    if (!q || !k || !v || !o || !offsets) return BSA_ERR_NULL_POINTER;
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || (reinterpret_cast<uintptr_t>(o) & 31)) return BSA_ERR_ALIGNMENT;
+    if (!q || !k || !v || !o || !offsets || (lse != nullptr) != (o_low != nullptr)) return BSA_ERR_NULL_POINTER;
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || (reinterpret_cast<uintptr_t>(o) & 31) || (reinterpret_cast<uintptr_t>(o_low) & 31)) return BSA_ERR_ALIGNMENT;
     if ((checked = check_strides(q_token_stride, q_head_stride)) != BSA_OK || (checked = check_strides(k_token_stride, k_head_stride)) != BSA_OK ||
         (checked = check_strides(v_token_stride, v_head_stride)) != BSA_OK) return checked;
     PackedParams p{};
-    p.o = o; p.lse = lse; p.offsets = offsets;
+    p.o = o; p.o_low = o_low; p.lse = lse; p.offsets = offsets;
     p.batch = (int)batch; p.rows = (int)rows; p.q_heads = (int)q_heads; p.kv_heads = (int)kv_heads;
     p.group = (int)(q_heads / kv_heads); p.causal = causal != 0;
     p.pair = p.group % 2 == 0;
@@ -457,14 +474,21 @@ extern "C" int bsa_packed_forward(int dtype, const void* q, int64_t q_token_stri
     // a scale of 0 stays a factor that keeps masked scores at -infinity
     p.scale_log2 = fmaxf(fabsf(scale) * kPackedLog2e, 1e-37f);
     p.status = static_cast<uint32_t*>(workspace);
-    CUtensorMap mq, mk, mv, mo;
+    CUtensorMap mq, mk, mv, mo, ml;
     if (!bind_device()) return BSA_ERR_LAUNCH;
     if (!make_packed_map(&mq, dtype, q, rows, q_heads, head_dim, q_token_stride, q_head_stride) ||
         !make_packed_map(&mk, dtype, k, rows, kv_heads, head_dim, k_token_stride, k_head_stride) ||
         !make_packed_map(&mv, dtype, v, rows, kv_heads, head_dim, v_token_stride, v_head_stride) ||
-        !make_packed_map(&mo, dtype, o, rows, q_heads, head_dim, q_heads * head_dim, head_dim, 32)) return BSA_ERR_DRIVER;
+        !make_packed_map(&mo, dtype, o, rows, q_heads, head_dim, q_heads * head_dim, head_dim, 32) ||
+        !make_packed_map(&ml, dtype, o_low ? o_low : o, rows, q_heads, head_dim, q_heads * head_dim, head_dim, 32)) return BSA_ERR_DRIVER;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == BSA_DTYPE_BF16)
-        return head_dim == 64 ? launch_forward<true, 64>(p, mq, mk, mv, mo, s) : launch_forward<true, 128>(p, mq, mk, mv, mo, s);
-    return head_dim == 64 ? launch_forward<false, 64>(p, mq, mk, mv, mo, s) : launch_forward<false, 128>(p, mq, mk, mv, mo, s);
+    const auto launch = [&](auto bf16, auto dim) {
+        constexpr bool kBf16 = decltype(bf16)::value;
+        constexpr int kDim = decltype(dim)::value;
+        return lse ? launch_forward<kBf16, kDim, true>(p, mq, mk, mv, mo, ml, s) : launch_forward<kBf16, kDim, false>(p, mq, mk, mv, mo, ml, s);
+    };
+    using D64 = std::integral_constant<int, 64>;
+    using D128 = std::integral_constant<int, 128>;
+    if (dtype == BSA_DTYPE_BF16) return head_dim == 64 ? launch(std::true_type{}, D64{}) : launch(std::true_type{}, D128{});
+    return head_dim == 64 ? launch(std::false_type{}, D64{}) : launch(std::false_type{}, D128{});
 }

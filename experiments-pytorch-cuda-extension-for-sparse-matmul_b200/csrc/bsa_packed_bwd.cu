@@ -31,6 +31,7 @@ constexpr int kBwdThreads = 384;
 
 struct PackedBwdParams {
     const void* o;
+    const void* o_low;                          // what rounding took from o
     const void* dout;
     int64_t dout_token, dout_head;              // strides in elements
     const float* lse;
@@ -45,7 +46,7 @@ struct PackedBwdParams {
     uint32_t* status;
 };
 
-// One row and head per D / 8 lanes.
+// One row and head per D / 8 lanes.  delta is made from o as it was before its rounding: with the rounded o alone the gradients' error against 64 bits is 1.5 times that of fp32 arithmetic rounded at the end.
 template <typename T, int kDim>
 __global__ void __launch_bounds__(256) packed_stats_kernel(const PackedBwdParams p) {
     constexpr int kLanes = kDim / 8;
@@ -58,10 +59,12 @@ __global__ void __launch_bounds__(256) packed_stats_kernel(const PackedBwdParams
     if (in) {
         const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.o) + at * kDim + lane * 8);
         const uint4 b = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.dout) + row * p.dout_token + head * p.dout_head + lane * 8);
+        const uint4 low = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.o_low) + at * kDim + lane * 8);
         const T* x = reinterpret_cast<const T*>(&a);
+        const T* z = reinterpret_cast<const T*>(&low);
         const T* y = reinterpret_cast<const T*>(&b);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(Scalar<T>::to_float(x[e]), Scalar<T>::to_float(y[e]), sum);
+        for (int e = 0; e < 8; ++e) sum = fmaf(Scalar<T>::to_float(x[e]) + Scalar<T>::to_float(z[e]), Scalar<T>::to_float(y[e]), sum);
     }
 #pragma unroll
     for (int s = kLanes / 2; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
@@ -679,7 +682,7 @@ int launch_backward(const PackedBwdParams& p, const CUtensorMap& mq, const CUten
 
 extern "C" int bsa_packed_backward(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                                    int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
-                                   int64_t v_head_stride, const void* o, const void* dout, int64_t dout_token_stride,
+                                   int64_t v_head_stride, const void* o, const void* o_low, const void* dout, int64_t dout_token_stride,
                                    int64_t dout_head_stride, const float* lse, void* dq, void* dk, void* dv,
                                    const int32_t* offsets, int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_heads,
                                    int64_t head_dim, float scale, int causal, void* stats, size_t stats_bytes,
@@ -689,8 +692,8 @@ extern "C" int bsa_packed_backward(int dtype, const void* q, int64_t q_token_str
     if (checked != BSA_OK) return checked;
     if (!workspace || workspace_bytes < BSA_WORKSPACE_BYTES) return BSA_ERR_WORKSPACE;
     if (rows == 0) return BSA_OK;
-    if (!q || !k || !v || !o || !dout || !lse || !dq || !dk || !dv || !offsets || !stats) return BSA_ERR_NULL_POINTER;
-    for (const void* ptr : {q, k, v, o, dout, static_cast<const void*>(stats)})
+    if (!q || !k || !v || !o || !o_low || !dout || !lse || !dq || !dk || !dv || !offsets || !stats) return BSA_ERR_NULL_POINTER;
+    for (const void* ptr : {q, k, v, o, o_low, dout, static_cast<const void*>(stats)})
         if (!aligned16(ptr)) return BSA_ERR_ALIGNMENT;
     for (const void* ptr : {dq, dk, dv})
         if (reinterpret_cast<uintptr_t>(ptr) & 31) return BSA_ERR_ALIGNMENT;
@@ -699,7 +702,7 @@ extern "C" int bsa_packed_backward(int dtype, const void* q, int64_t q_token_str
         (checked = check_strides(dout_token_stride, dout_head_stride)) != BSA_OK) return checked;
     if (stats_bytes < (size_t)rows * q_heads * sizeof(float2)) return BSA_ERR_WORKSPACE;
     PackedBwdParams p{};
-    p.o = o; p.dout = dout; p.dout_token = dout_token_stride; p.dout_head = dout_head_stride;
+    p.o = o; p.o_low = o_low; p.dout = dout; p.dout_token = dout_token_stride; p.dout_head = dout_head_stride;
     p.lse = lse; p.stats = static_cast<float2*>(stats);
     p.dq = dq; p.dk = dk; p.dv = dv; p.offsets = offsets;
     p.batch = (int)batch; p.rows = (int)rows; p.q_heads = (int)q_heads; p.kv_heads = (int)kv_heads;

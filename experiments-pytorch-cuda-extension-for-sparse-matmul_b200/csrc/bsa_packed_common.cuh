@@ -212,24 +212,32 @@ __device__ __forceinline__ void store_row32(void* to, const uint32_t (&r)[32], f
 // swizzled) and a TMA store where all 32 rows belong to the sequence, else row by row.  (A row per thread stored straight
 // from registers touches 32 lines per instruction: an epilogue of 128 x 128 took 3000-4000 cycles.)
 __device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-template <bool kBf16>
-__device__ __forceinline__ void store_rows64(uint8_t* stage, const CUtensorMap* map, const uint32_t (&r)[2][32], float by, int column,
-                                             int head, int row, int lane) {
+__device__ __forceinline__ void store_rows64(uint8_t* stage, const CUtensorMap* map, const uint32_t (&w)[32], int column, int head,
+                                             int row, int lane) {
     if (lane == 0) store_done();                // the last store has read the stage
     __syncwarp();
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            w[e] = pack2<kBf16>(__uint_as_float(r[u / 4][8 * (u % 4) + 2 * e]) * by, __uint_as_float(r[u / 4][8 * (u % 4) + 2 * e + 1]) * by);
-        *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+    for (int u = 0; u < 8; ++u)
+        *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
     fence_async_shared();
     __syncwarp();
     if (lane == 0)
         asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];\n\tcp.async.bulk.commit_group;"
                      ::"l"(map), "r"(smem_u32(stage)), "r"(column), "r"(head), "r"(row) : "memory");
+}
+// The same 64 columns of one row from its thread (32-byte aligned).
+__device__ __forceinline__ void store_row64(void* to, const uint32_t (&w)[32]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const uint32_t part[8] = {w[8 * q], w[8 * q + 1], w[8 * q + 2], w[8 * q + 3], w[8 * q + 4], w[8 * q + 5], w[8 * q + 6], w[8 * q + 7]};
+        st_global_v8(static_cast<uint8_t*>(to) + 32 * q, part);
+    }
+}
+// Two values that a word of 16-bit values stands for.
+template <bool kBf16>
+__device__ __forceinline__ float2 word_values(uint32_t w) {
+    if (kBf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
 // Zero rows [from, to) of a contiguous 16-bit [rows, heads, head_dim] tensor, one head, by thread `me` of `threads`.

@@ -554,31 +554,39 @@ void check_packed(const torch::Tensor& q, const torch::Tensor& k, const torch::T
                 offsets.is_contiguous(), "offsets must be a contiguous int32 tensor [sequences + 1] on q's device");
 }
 
-// (o, lse) of attention inside the sequences of a packed batch; lse [heads, rows] in units of log2.
-std::tuple<torch::Tensor, torch::Tensor> packed_attention_forward(torch::Tensor q, torch::Tensor k, torch::Tensor v,
-                                                                  torch::Tensor offsets, double scale, bool causal) {
+// (o, lse, o_low) of attention inside the sequences of a packed batch; lse [heads, rows] in units of log2, o_low what
+// rounding took from o (lse and o_low for the backward only, else empty).
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attention_forward(
+        torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor offsets, double scale, bool causal, bool for_backward) {
     check_packed(q, k, v, offsets);
     c10::cuda::CUDAGuard guard(q.device());
     auto o = torch::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
-    auto lse = torch::empty({q.size(1), q.size(0)}, q.options().dtype(torch::kFloat));
+    torch::Tensor lse, o_low;
+    if (for_backward) {
+        lse = torch::empty({q.size(1), q.size(0)}, q.options().dtype(torch::kFloat));
+        o_low = torch::empty_like(o);
+    }
     if (q.size(0) > 0) {
         q = map_ready(q); k = map_ready(k); v = map_ready(v);
         auto ws = workspace_for(q.device());
         check_status(bsa_packed_forward(dtype_code(q), q.data_ptr(), map_stride(q, 0), map_stride(q, 1), k.data_ptr(),
                                         map_stride(k, 0), map_stride(k, 1), v.data_ptr(), map_stride(v, 0), map_stride(v, 1),
-                                        o.data_ptr(), lse.data_ptr<float>(), offsets.data_ptr<int>(), q.size(0),
+                                        o.data_ptr(), for_backward ? o_low.data_ptr() : nullptr,
+                                        for_backward ? lse.data_ptr<float>() : nullptr, offsets.data_ptr<int>(), q.size(0),
                                         offsets.size(0) - 1, q.size(1), k.size(1), q.size(2), static_cast<float>(scale), causal,
                                         ws.data_ptr(), BSA_WORKSPACE_BYTES, at::cuda::getCurrentCUDAStream().stream()),
                      "packed_attention_forward");
     }
-    return {o, lse};
+    return {o, lse, o_low};
 }
 
 // (dq, dk, dv) from the inputs, the forward's results and the output's gradient.
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attention_backward(
-        torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor dout, torch::Tensor lse,
-        torch::Tensor offsets, double scale, bool causal) {
+        torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor o_low, torch::Tensor dout,
+        torch::Tensor lse, torch::Tensor offsets, double scale, bool causal) {
     check_packed(q, k, v, offsets);
+    TORCH_CHECK(o_low.sizes() == q.sizes() && o_low.scalar_type() == q.scalar_type() && o_low.device() == q.device() &&
+                o_low.is_contiguous(), "o_low must be the forward's");
     TORCH_CHECK(o.sizes() == q.sizes() && dout.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() &&
                 dout.scalar_type() == q.scalar_type() && o.device() == q.device() && dout.device() == q.device(),
                 "o and dout must have q's shape, dtype and device");
@@ -593,7 +601,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attention_backwar
         auto stats = torch::empty({q.size(1), q.size(0), 2}, q.options().dtype(torch::kFloat));
         check_status(bsa_packed_backward(dtype_code(q), q.data_ptr(), map_stride(q, 0), map_stride(q, 1), k.data_ptr(),
                                          map_stride(k, 0), map_stride(k, 1), v.data_ptr(), map_stride(v, 0), map_stride(v, 1),
-                                         o.data_ptr(), dout.data_ptr(), map_stride(dout, 0), map_stride(dout, 1),
+                                         o.data_ptr(), o_low.data_ptr(), dout.data_ptr(), map_stride(dout, 0), map_stride(dout, 1),
                                          lse.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                          offsets.data_ptr<int>(), q.size(0), offsets.size(0) - 1, q.size(1), k.size(1), q.size(2),
                                          static_cast<float>(scale), causal, stats.data_ptr(), static_cast<size_t>(stats.numel()) * 4,
@@ -653,11 +661,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("lengths"), py::arg("counts") = py::none(), py::arg("tree") = py::none(), py::arg("scale") = 1.0,
           py::arg("pattern") = py::none(), py::arg("pattern_block") = 0);
     m.def("packed_attention_forward", &packed_attention_forward,
-          "Attention inside the sequences of a packed batch; returns (output, log2-sum-exp).", py::arg("q"), py::arg("k"),
-          py::arg("v"), py::arg("offsets"), py::arg("scale") = 1.0, py::arg("causal") = true);
+          "Attention inside the sequences of a packed batch; returns (output, log2-sum-exp, rest of the output).",
+          py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"), py::arg("scale") = 1.0, py::arg("causal") = true,
+          py::arg("for_backward") = true);
     m.def("packed_attention_backward", &packed_attention_backward, "Its gradients (dq, dk, dv).", py::arg("q"), py::arg("k"),
-          py::arg("v"), py::arg("o"), py::arg("dout"), py::arg("lse"), py::arg("offsets"), py::arg("scale") = 1.0,
-          py::arg("causal") = true);
+          py::arg("v"), py::arg("o"), py::arg("o_low"), py::arg("dout"), py::arg("lse"), py::arg("offsets"),
+          py::arg("scale") = 1.0, py::arg("causal") = true);
     m.def("check_device_status", &check_device_status, "Synchronise the device's current stream; raise if a kernel reported a time-out or a bad block descriptor since the last check.",
           py::arg("device_index") = 0);
     m.def("version", []() { return bsa_version(); });

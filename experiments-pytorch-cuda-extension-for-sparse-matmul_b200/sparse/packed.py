@@ -10,7 +10,8 @@ groups of query heads may share a key head.  The reference has no such op.
 Nothing about the lengths is read on the host: a captured CUDA graph follows
 ``offsets`` that change in place, as long as the number of rows stays.
 
-The forward keeps the output and the rows' log-sum-exp; the backward recomputes
+The forward keeps the output, what its rounding to 16 bits took (so that
+rowsum(dO o O) is exact to fp32) and the rows' log-sum-exp; the backward recomputes
 the probabilities on chip, by key tiles for dK and dV (summed over the heads
 that share a key head) and by query tiles for dQ, without atomics: gradients
 repeat bit for bit.
@@ -26,15 +27,17 @@ class PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, scale: float = 1.0,
                 causal: bool = True) -> torch.Tensor:
-        out, lse = kernel.sparse_ops.packed_attention_forward(q, k, v, offsets, float(scale), bool(causal))
-        ctx.save_for_backward(q, k, v, out, lse, offsets)
+        keep = any(ctx.needs_input_grad[:3])
+        out, lse, low = kernel.sparse_ops.packed_attention_forward(q, k, v, offsets, float(scale), bool(causal), keep)
+        if keep:
+            ctx.save_for_backward(q, k, v, out, low, lse, offsets)
         ctx.scale, ctx.causal = float(scale), bool(causal)
         return kernel.check(out)
 
     @staticmethod
     def backward(ctx: Any, dout: torch.Tensor) -> Tuple[Optional[torch.Tensor], ...]:
-        q, k, v, out, lse, offsets = ctx.saved_tensors
-        dq, dk, dv = kernel.sparse_ops.packed_attention_backward(q, k, v, out, dout, lse, offsets, ctx.scale, ctx.causal)
+        q, k, v, out, low, lse, offsets = ctx.saved_tensors
+        dq, dk, dv = kernel.sparse_ops.packed_attention_backward(q, k, v, out, low, dout, lse, offsets, ctx.scale, ctx.causal)
         kernel.check(dout)
         return dq, dk, dv, None, None, None
 

@@ -244,20 +244,22 @@ int bsa_attention_backward(int dtype, const void* q, const void* k, const void* 
  *                   outside the tensors; the output is then not defined.
  *   causal          nonzero: a row sees its own and earlier rows of its sequence
  *   lse             float [q_heads, rows]: log2 of the row sums of
- *                   exp(scale * s), -inf for rows behind the last sequence (forward:
- *                   may be NULL)
+ *                   exp(scale * s), -inf for rows behind the last sequence
+ *   o_low           o's shape and type: what rounding took from o, for the backward's
+ *                   rowsum(dout o O).  The forward writes both where a backward
+ *                   follows; give NULL for both where none does.
  *   stats           scratch of rows * q_heads * 8 bytes, 16-byte aligned
  * BSA_DTYPE_F16 / BSA_DTYPE_BF16, head_dim 64 or 128.
  */
 int bsa_packed_forward(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                        int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
-                       int64_t v_head_stride, void* o, float* lse, const int32_t* offsets, int64_t rows,
+                       int64_t v_head_stride, void* o, void* o_low, float* lse, const int32_t* offsets, int64_t rows,
                        int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scale, int causal,
                        void* workspace, size_t workspace_bytes, void* stream);
 int bsa_packed_backward(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                         int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
-                        int64_t v_head_stride, const void* o, const void* dout, int64_t dout_token_stride,
-                        int64_t dout_head_stride, const float* lse, void* dq, void* dk, void* dv,
+                        int64_t v_head_stride, const void* o, const void* o_low, const void* dout,
+                        int64_t dout_token_stride, int64_t dout_head_stride, const float* lse, void* dq, void* dk, void* dv,
                         const int32_t* offsets, int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_heads,
                         int64_t head_dim, float scale, int causal, void* stats, size_t stats_bytes,
                         void* workspace, size_t workspace_bytes, void* stream);

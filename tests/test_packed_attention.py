@@ -20,26 +20,27 @@ def test_packed_validation_codes():
     lib = ctypes.CDLL(path)
     i, p, z = ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t
     f = lib.bsa_packed_forward
-    f.argtypes = [ctypes.c_int] + [p, i, i] * 3 + [p, p, p] + [i] * 5 + [ctypes.c_float, ctypes.c_int, p, z, p]
+    f.argtypes = [ctypes.c_int] + [p, i, i] * 3 + [p, p, p, p] + [i] * 5 + [ctypes.c_float, ctypes.c_int, p, z, p]
 
-    def call(dtype=1, q=32, strides=(1024, 128), o=32, offsets=16, rows=10, batch=1, heads=8, kv=4, dim=128, ws=16, ws_bytes=256):
-        return f(dtype, q, *strides, 32, *strides, 32, *strides, o, 32, offsets, rows, batch, heads, kv, dim, 1.0, 1, ws, ws_bytes, None)
+    def call(dtype=1, q=32, strides=(1024, 128), o=32, offsets=16, rows=10, batch=1, heads=8, kv=4, dim=128, ws=16, ws_bytes=256, low=32):
+        return f(dtype, q, *strides, 32, *strides, 32, *strides, o, low, 32, offsets, rows, batch, heads, kv, dim, 1.0, 1, ws, ws_bytes, None)
 
     assert call(dtype=0) == 3 and call(dim=96) == 4 and call(heads=6) == 4 and call(kv=0) == 4 and call(rows=-1) == 4
     assert call(batch=-1) == 4 and call(rows=2 ** 31) == 10 and call(rows=2 ** 30, heads=65532, kv=4) == 10
+    assert call(low=None) == 1 and call(low=48) == 6             # lse without the rest of o
     assert call(q=None) == 1 and call(o=None) == 1 and call(offsets=None) == 1
     assert call(q=24) == 6 and call(o=16) == 6 and call(strides=(1023, 128)) == 6 and call(strides=(0, 128)) == 4
     assert call(ws=None) == 7 and call(ws_bytes=0) == 7
     assert call(rows=0) == 0
 
     g = lib.bsa_packed_backward
-    g.argtypes = [ctypes.c_int] + [p, i, i] * 3 + [p, p, i, i] + [p] * 5 + [i] * 5 + [ctypes.c_float, ctypes.c_int, p, z, p, z, p]
+    g.argtypes = [ctypes.c_int] + [p, i, i] * 3 + [p, p, p, i, i] + [p] * 5 + [i] * 5 + [ctypes.c_float, ctypes.c_int, p, z, p, z, p]
 
-    def back(dtype=1, dout=32, dk=32, lse=32, rows=10, heads=8, stats=32, stats_bytes=1 << 20):
-        return g(dtype, 32, 1024, 128, 32, 512, 128, 32, 512, 128, 32, dout, 1024, 128, lse, 32, dk, 32, 32, rows, 1, heads, 4, 128,
+    def back(dtype=1, dout=32, dk=32, lse=32, rows=10, heads=8, stats=32, stats_bytes=1 << 20, low=32):
+        return g(dtype, 32, 1024, 128, 32, 512, 128, 32, 512, 128, 32, low, dout, 1024, 128, lse, 32, dk, 32, 32, rows, 1, heads, 4, 128,
                  1.0, 1, stats, stats_bytes, 16, 256, None)
 
-    assert back(dtype=0) == 3 and back(heads=9) == 4 and back(dout=None) == 1 and back(lse=None) == 1 and back(stats=None) == 1
+    assert back(dtype=0) == 3 and back(heads=9) == 4 and back(dout=None) == 1 and back(lse=None) == 1 and back(low=None) == 1 and back(stats=None) == 1
     assert back(dk=48) == 6 and back(stats_bytes=10 * 8 * 8 - 1) == 7 and back(rows=0) == 0
 
 
