@@ -625,6 +625,38 @@ void check_device_status(int64_t device_index) {
                  "check_device_status");
 }
 
+// packed_attention as an autograd op.  It lives here and not in Python because a small step (a few hundred rows) is bound by
+// the host: the backward then runs without the interpreter.  `check`: read the device status after each pass.
+class PackedAttention : public torch::autograd::Function<PackedAttention> {
+public:
+    static torch::Tensor forward(torch::autograd::AutogradContext* ctx, torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                                 torch::Tensor offsets, double scale, bool causal, bool check) {
+        auto [out, lse, low] = packed_attention_forward(q, k, v, offsets, scale, causal, true);
+        ctx->save_for_backward({q, k, v, out, low, lse, offsets});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["causal"] = causal;
+        ctx->saved_data["check"] = check;
+        return out;
+    }
+    static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "packed_attention has no second derivative (create_graph=True)");
+        const auto saved = ctx->get_saved_variables();
+        auto [dq, dk, dv] = packed_attention_backward(saved[0], saved[1], saved[2], saved[3], saved[4], grads[0], saved[5], saved[6],
+                                                      ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool());
+        if (ctx->saved_data["check"].toBool()) check_device_status(dq.device().index());
+        return {dq, dk, dv, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()};
+    }
+};
+
+torch::Tensor packed_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor offsets, double scale, bool causal,
+                               bool check) {
+    const bool learns = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+    auto out = learns ? PackedAttention::apply(q, k, v, offsets, scale, causal, check)
+                      : std::get<0>(packed_attention_forward(q, k, v, offsets, scale, causal, false));
+    if (check) check_device_status(q.device().index());
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -660,6 +692,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("keys"), py::arg("values"), py::arg("key_scales"), py::arg("value_scales"), py::arg("table"),
           py::arg("lengths"), py::arg("counts") = py::none(), py::arg("tree") = py::none(), py::arg("scale") = 1.0,
           py::arg("pattern") = py::none(), py::arg("pattern_block") = 0);
+    m.def("packed_attention", &packed_attention, "Attention inside the sequences of a packed batch (an autograd op).",
+          py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"), py::arg("scale") = 1.0, py::arg("causal") = true,
+          py::arg("check") = false, py::call_guard<py::gil_scoped_release>());
     m.def("packed_attention_forward", &packed_attention_forward,
           "Attention inside the sequences of a packed batch; returns (output, log2-sum-exp, rest of the output).",
           py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"), py::arg("scale") = 1.0, py::arg("causal") = true,

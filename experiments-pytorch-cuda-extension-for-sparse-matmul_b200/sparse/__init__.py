@@ -12,11 +12,11 @@ from .matmul import matmul, SparseMatMul
 from .softmax import softmax, SparseSoftmax
 from .attention import attention, SparseAttention
 from .module import BlockSparseSelfAttention
-from .packed import packed_attention, PackedAttention
+from .packed import packed_attention
 from .cache import Cache, cache_read, cache_slots, cache_write, make_cache
 from .cached_attention import cached_attention, tree_words
 from .batched import BatchedSparseLayout, batched_matmul, batched_softmax, batched_attention
 
 __all__ = ["SparseLayout", "matmul", "SparseMatMul", "softmax", "SparseSoftmax", "attention", "SparseAttention", "BlockSparseSelfAttention",
-           "packed_attention", "PackedAttention", "Cache", "cache_read", "cache_slots", "cache_write", "make_cache", "cached_attention", "tree_words",
+           "packed_attention", "Cache", "cache_read", "cache_slots", "cache_write", "make_cache", "cached_attention", "tree_words",
            "BatchedSparseLayout", "batched_matmul", "batched_softmax", "batched_attention"]

@@ -14,32 +14,11 @@ The forward keeps the output, what its rounding to 16 bits took (so that
 rowsum(dO o O) is exact to fp32) and the rows' log-sum-exp; the backward recomputes
 the probabilities on chip, by key tiles for dK and dV (summed over the heads
 that share a key head) and by query tiles for dQ, without atomics: gradients
-repeat bit for bit.
+repeat bit for bit.  There is no second derivative.
 """
-from typing import Any, Optional, Tuple
-
 import torch
 
 from . import kernel
-
-
-class PackedAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx: Any, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, scale: float = 1.0,
-                causal: bool = True) -> torch.Tensor:
-        keep = any(ctx.needs_input_grad[:3])
-        out, lse, low = kernel.sparse_ops.packed_attention_forward(q, k, v, offsets, float(scale), bool(causal), keep)
-        if keep:
-            ctx.save_for_backward(q, k, v, out, low, lse, offsets)
-        ctx.scale, ctx.causal = float(scale), bool(causal)
-        return kernel.check(out)
-
-    @staticmethod
-    def backward(ctx: Any, dout: torch.Tensor) -> Tuple[Optional[torch.Tensor], ...]:
-        q, k, v, out, low, lse, offsets = ctx.saved_tensors
-        dq, dk, dv = kernel.sparse_ops.packed_attention_backward(q, k, v, out, low, dout, lse, offsets, ctx.scale, ctx.causal)
-        kernel.check(dout)
-        return dq, dk, dv, None, None, None
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, scale: float = 1.0,
@@ -51,4 +30,4 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     (it may be empty); ``offsets[0]`` is 0.  Rows behind the last sequence give zeros, and zero gradients.  Offsets that
     decrease or pass the last row are reported by ``check_device_status``.  A NaN or an infinity reaches rows of its own
     sequence only."""
-    return PackedAttention.apply(q, k, v, offsets, scale, causal)
+    return kernel.sparse_ops.packed_attention(q, k, v, offsets, float(scale), bool(causal), kernel.debug_checks)

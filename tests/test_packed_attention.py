@@ -318,6 +318,39 @@ def test_gpu_refusals():
                        (x, x[:, :0], x[:, :0], offsets)):
         with pytest.raises(RuntimeError):
             packed_attention(q, k, v, o)
+    a = x.clone().requires_grad_()
+    out = packed_attention(a, a, a, offsets)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(out.sum(), a, create_graph=True)
+    _status()
+
+
+@pytest.mark.gpu
+def test_which_inputs_learn_and_debug_checks():
+    from sparse import kernel, packed_attention
+    lengths = [90, 41]
+    q, k, v, do, offsets = _inputs(lengths, 0, 4, 2, 64, torch.bfloat16, 13)
+    want = _run(q, k, v, do, offsets, 0.125, True)
+    q, k, v, do, offsets = (t.cuda() for t in (q, k, v, do, offsets))
+    with torch.no_grad():
+        assert not packed_attention(q.requires_grad_(), k, v, offsets, 0.125).requires_grad
+    q.requires_grad_(False)
+    assert not packed_attention(q, k, v, offsets, 0.125).requires_grad
+    for learns in range(3):
+        x = [t.detach().requires_grad_(i == learns) for i, t in enumerate((q, k, v))]
+        out = packed_attention(*x, offsets, 0.125)
+        out.backward(do)
+        assert torch.equal(out, want[0])
+        for i in range(3):
+            assert torch.equal(x[i].grad, want[1 + i]) if i == learns else x[i].grad is None
+    kernel.debug_checks = True
+    try:
+        x = [t.detach().requires_grad_() for t in (q, k, v)]
+        packed_attention(*x, offsets, 0.125).backward(do)
+        with pytest.raises(RuntimeError):
+            packed_attention(*x, torch.tensor([0, 200], dtype=torch.int32, device="cuda"))
+    finally:
+        kernel.debug_checks = False
     _status()
 
 
