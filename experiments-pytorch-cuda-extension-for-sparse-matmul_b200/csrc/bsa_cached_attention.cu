@@ -28,7 +28,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "bsa_tc_common.cuh"
+#include "bsa_cached_common.cuh"
 
 namespace bsa {
 namespace {
@@ -37,29 +37,7 @@ constexpr int kTileKeys = 64;
 constexpr int kConsumers = 4;                   // warps
 constexpr int kBegin = 6;                       // what beginning and ending a (sequence, head) costs a CTA, in tiles
 constexpr float kLog2e = 1.4426950408889634f;
-
-struct CachedParams {
-    const void* q;
-    void* o;
-    int64_t q_batch, q_draft, q_head;           // strides of q in elements
-    const float* scales[2];
-    const int32_t* table;
-    const int32_t* lengths;
-    const int32_t* counts;                      // may be null
-    const int64_t* tree;                        // may be null
-    const uint8_t* pattern;                     // may be null: [pattern_rows, pattern_cols] of 1 << pattern_shift tokens
-    int pattern_rows, pattern_cols, pattern_shift;
-    int batch, drafts, group, kv_heads, row_tiles, table_width, pages, page_shift;
-    float scale_log2;                           // scale * log2 e
-    float* partial;                             // [ctas][2][rows][head_dim], then [ctas][2][rows][2] of (m, l)
-    int ctas;
-    uint32_t* status;
-};
-
-struct Share {
-    int64_t per, first, end;        // units per CTA; this CTA's range
-    int b, hm, tile;                // where the range starts
-};
+constexpr int64_t kWideRows = 32;               // query rows of a key head above which a 16-bit cache goes to the tcgen05 kernel
 
 template <int kStages>
 struct __align__(8) CachedBarriers {
@@ -68,79 +46,6 @@ struct __align__(8) CachedBarriers {
     Share share;
     int abort_flag;
 };
-
-__device__ __forceinline__ int cached_length(const CachedParams& p, int b) {
-    return min(max(p.lengths[b], 0), p.table_width << p.page_shift);
-}
-__device__ __forceinline__ int cached_tiles(const CachedParams& p, int b) {
-    return max(1, (cached_length(p, b) + kTileKeys - 1) / kTileKeys);
-}
-
-// Units of one head and row tile of the whole batch, and of the sequences before `part` (in `before`), by one warp.
-__device__ __forceinline__ int64_t total_cost(const CachedParams& p, int part, int64_t& before, int lane) {
-    int64_t sum = 0, some = 0;
-#pragma unroll 4
-    for (int b = lane; b < p.batch; b += 32) {
-        const int cost = cached_tiles(p, b) + kBegin;
-        sum += cost;
-        if (b < part) some += cost;
-    }
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, s);
-        some += __shfl_xor_sync(0xffffffffu, some, s);
-    }
-    before = some;
-    return sum;
-}
-// a / b; the units fit 32 bits unless a batch holds more keys than the device's memory
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-    return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
-}
-
-// A (sequence, head, row tile) takes kBegin + tiles units of the list, its tiles last.  Finds where this CTA's share
-// starts; a share that starts inside the first kBegin units starts at tile 0.
-__device__ __forceinline__ Share find_share(const CachedParams& p, int cta, int lane) {
-    Share s;
-    const int hms = p.kv_heads * p.row_tiles;
-    // (the first 32 sequences stay in registers: with no more than those there is one load on the way to the first tile)
-    const int first = lane < p.batch ? cached_tiles(p, lane) + kBegin : 0;
-    int64_t sum = first;
-    for (int b = 32 + lane; b < p.batch; b += 32) sum += cached_tiles(p, b) + kBegin;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    const int64_t units = sum * hms;
-    s.per = quotient(units + p.ctas - 1, p.ctas);
-    s.first = min((int64_t)cta * s.per, units);
-    s.end = min(s.first + s.per, units);
-    s.b = s.hm = s.tile = 0;
-    if (s.first >= s.end) return s;
-    int64_t before = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += 32) {
-        const int mine = b0 == 0 ? first : (b0 + lane < p.batch ? cached_tiles(p, b0 + lane) + kBegin : 0);
-        int64_t upto = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int64_t o = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += o;
-        }
-        const uint32_t past = __ballot_sync(0xffffffffu, s.first < (before + upto) * hms);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            const int cost = __shfl_sync(0xffffffffu, mine, l);
-            const int64_t start = before + __shfl_sync(0xffffffffu, upto, l) - cost;
-            const int64_t off = s.first - start * hms;
-            s.b = b0 + l;
-            s.hm = (int)quotient(off, cost);
-            const int within = (int)(off - (int64_t)s.hm * cost);
-            s.tile = max(within - kBegin, 0);
-            s.first += max(kBegin - within, 0);             // the unit of that tile
-            return s;
-        }
-        before += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    return s;
-}
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -219,7 +124,7 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
     Bars* bars = reinterpret_cast<Bars*>(merge + S::kJoinFloats);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0) {
-        const Share mine = find_share(p, (int)blockIdx.x, lane);
+        const Share mine = find_share<kTileKeys, kBegin>(p, (int)blockIdx.x, lane);
         if (lane == 0) bars->share = mine;
     } else if (warp == kConsumers && lane == 0) {
         bars->abort_flag = 0;
@@ -687,8 +592,8 @@ cached_join_kernel(const CachedParams p, int rows) {
     const int head = hm / p.row_tiles, row = (hm - head * p.row_tiles) * rows + r, draft = row / p.group;
     // which CTAs hold this item's tiles follows from the lengths alone: found while the main kernel still runs
     int64_t before;
-    const int64_t per = quotient(total_cost(p, b, before, lane) * hms + p.ctas - 1, p.ctas);
-    const int tiles = cached_tiles(p, b);
+    const int64_t per = quotient(total_cost<kTileKeys, kBegin>(p, b, before, lane) * hms + p.ctas - 1, p.ctas);
+    const int tiles = cached_tiles<kTileKeys>(p, b);
     const int64_t start = before * hms + (int64_t)hm * (tiles + kBegin) + kBegin;       // the unit of tile 0
     const int first = (int)quotient(start, per), last = (int)quotient(start + tiles - 1, per);
     // (also where there is nothing to do: the stream's next kernel waits for this grid, which must not end before the main one)
@@ -734,22 +639,6 @@ cached_join_kernel(const CachedParams p, int rows) {
     for (int e = 0; e < kCols; ++e) to[e] = Scalar<T>::from_float(sum[e] * inv);
 }
 
-// Map of a side of the cache as rows of head_dim elements, one page (at most a tile of it) per box.
-bool make_cache_map(CUtensorMap* map, int store, int dtype, const void* base, int64_t rows, int64_t dim, int piece) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) return false;
-    const int es = store == BSA_CACHE_E4M3 ? 1 : 2, row_bytes = (int)dim * es, panel = row_bytes < 128 ? row_bytes : 128;
-    const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)rows, 1};
-    const cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)row_bytes * (cuuint64_t)rows};
-    const cuuint32_t box[3] = {(cuuint32_t)(panel / es), (cuuint32_t)piece, 1};
-    const cuuint32_t elem[3] = {1, 1, 1};
-    const CUtensorMapDataType type = es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                                             : (dtype == BSA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
-    return fn(map, type, 3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              panel == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 int row_groups(int64_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
 
 template <typename T, bool kE4m3, int kDim, int kGroups>
@@ -793,7 +682,8 @@ int launch_cached_typed(int store, int64_t dim, int groups, const CachedParams& 
 extern "C" size_t bsa_cached_attention_scratch(int64_t drafts, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
     if (drafts <= 0 || kv_heads <= 0 || q_heads < kv_heads || head_dim <= 0) return 0;
     const int64_t rows = drafts * (q_heads / kv_heads), tile = 16 * bsa::row_groups(rows);
-    return (size_t)std::max(bsa::sm_count(), 1) * 2 * 2 * tile * (size_t)(head_dim + 2) * 4;
+    const size_t wide = rows > bsa::kWideRows ? bsa::cached_wide_scratch(head_dim) : 0;
+    return std::max(wide, (size_t)std::max(bsa::sm_count(), 1) * 2 * 2 * tile * (size_t)(head_dim + 2) * 4);
 }
 
 extern "C" int bsa_cached_attention(int dtype, int store, const void* q, int64_t q_batch_stride, int64_t q_draft_stride,
@@ -843,6 +733,8 @@ extern "C" int bsa_cached_attention(int dtype, int store, const void* q, int64_t
     // the driver's encoder needs the device's context bound to this thread
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) { cudaGetLastError(); return BSA_ERR_LAUNCH; }
+    if (drafts * group > kWideRows && store == BSA_CACHE_SAME && !pattern)
+        return cached_wide(p, dtype, head_dim, keys, values, page, static_cast<cudaStream_t>(stream));
     CUtensorMap map_k, map_v;
     const int64_t rows = pages * kv_heads * page;
     const int piece = (int)std::min<int64_t>(page, kTileKeys);

@@ -408,6 +408,10 @@ ATTENTION = [
     (64, 64, 2, 1, 64, [64, 130, 500], None, True),
     (128, 32, 5, 2, 33, [33, 100], [33, 7], False),
     (64, 128, 1, 16, 13, [2500, 13], None, True),
+    # many query rows per key head: lengths around a tile of 128 keys, one and several tiles per share, empty sequences
+    (128, 16, 1, 16, 3, [1, 2, 3, 127, 128, 129, 255, 256, 257, 0, 700], None, False),
+    (64, 64, 8, 8, 8, [50, 3000, 8, 0, 131] * 9, [8, 3, 8, 0, 1] * 9, True),
+    (128, 128, 4, 5, 60, [60, 61, 9000], None, True),
 ]
 
 
@@ -462,10 +466,11 @@ def test_cached_attention_with_a_layout(block, drafts, tree):
 
 
 @pytest.mark.gpu
-def test_cached_attention_pages_that_are_none():
+@pytest.mark.parametrize("store,group,drafts", [("same", 2, 1), ("same", 8, 8), ("e4m3", 4, 2)])
+def test_cached_attention_pages_that_are_none(store, group, drafts):
     """A page id outside the cache leaves its keys out and is reported; other sequences are not touched."""
     from sparse.kernel import sparse_ops
-    case = _Case(torch.float16, "same", 64, 16, 2, 2, 1, [100, 70], seed=2)
+    case = _Case(torch.float16, store, 64, 16, 2, group, drafts, [100, 70], seed=2)
     good = case.call()
     for bad in (-1, 10 ** 6, 2 ** 31 - 1, -2 ** 31):
         table = case.table.clone()
