@@ -25,6 +25,7 @@ namespace {
 constexpr int kWideBegin = 3;                   // what beginning and ending a (sequence, head) costs, in tiles
 constexpr int kWideStages = 3;
 constexpr int kWideThreads = 320;
+constexpr int kJoinCols = 4;
 
 struct __align__(16) WideBarriers {
     uint64_t q_full, q_empty, k_full[kWideStages], k_empty[kWideStages], v_full[kWideStages], v_empty[kWideStages];
@@ -38,6 +39,9 @@ struct __align__(16) WideBarriers {
 };
 template <int kDim>
 constexpr int wide_smem() { return (1 + 2 * kWideStages) * (kDim / 64) * kPanelBytes + (int)sizeof(WideBarriers); }
+
+// The lowest n bits.
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
 
 // The share of a CTA, segment by segment: tiles of one (sequence, head, row tile).
 struct Walk {
@@ -119,12 +123,17 @@ cached_wide_kernel(const CachedParams p, const __grid_constant__ CUtensorMap map
         for (; ok && w.more(); w.next(p)) {
             if (lane == 0 && p.lengths[w.b] != w.length) atomicExch(p.status, (uint32_t)BSA_ERR_BAD_SHAPE);
             const int head = w.hm / p.row_tiles, n = w.count();
-            for (int i = 0; ok && i < n; ++i, ++t) {
+            auto look = [&](int i) {                            // this lane's page of a tile, fetched a tile ahead
                 const int key = (w.tile + i) * kRowsTile + my_piece * piece;
+                return my_piece < pieces && i < n && key < w.length ? p.table[(int64_t)w.b * p.table_width + (key >> p.page_shift)] : 0;
+            };
+            int next = look(0);
+            for (int i = 0; ok && i < n; ++i, ++t) {
+                const int key = (w.tile + i) * kRowsTile + my_piece * piece, id = next;
+                next = look(i + 1);
                 bool there = my_piece < pieces && key < w.length;
                 int row = 0;
                 if (there) {
-                    const int id = p.table[(int64_t)w.b * p.table_width + (key >> p.page_shift)];
                     if ((uint32_t)id >= (uint32_t)p.pages) {
                         atomicExch(p.status, (uint32_t)BSA_ERR_BAD_SHAPE);
                         there = false;
@@ -241,6 +250,10 @@ cached_wide_kernel(const CachedParams p, const __grid_constant__ CUtensorMap map
                 uint4 x[kDim / 8];
 #pragma unroll
                 for (int i = 0; i < kDim / 8; ++i) x[i] = row_on ? *reinterpret_cast<const uint4*>(q + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+                if (negative) {                 // a negative scale: the queries' signs
+#pragma unroll
+                    for (int i = 0; i < kDim / 8; ++i) x[i] = make_uint4(x[i].x ^ 0x80008000u, x[i].y ^ 0x80008000u, x[i].z ^ 0x80008000u, x[i].w ^ 0x80008000u);
+                }
                 // their place is free once the last scores are made, and all of this stream have read what the other left there
                 ok = wait_all(&bars->q_empty, ((uint32_t)segment & 1u) ^ 1u, abort_flag, p.status) &&
                      wait_all(&bars->m_empty, ((uint32_t)m_no & 1u) ^ 1u, abort_flag, p.status);
@@ -261,23 +274,21 @@ cached_wide_kernel(const CachedParams p, const __grid_constant__ CUtensorMap map
 #pragma unroll
                 for (int q = 0; q < 4; ++q) tc_ld_32x32b_x32(s_tmem + (uint32_t)(32 * q), x[q]);
                 tc_wait_ld();
-                if (negative) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) x[q][e] ^= 0x80000000u;
-                }
                 const int key0 = (w.tile + i) * kRowsTile;
                 const uint32_t loaded = bars->ok[(t + i) & 7];
                 if (key0 + kRowsTile > prefix || __popc(loaded) != pieces) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
+                    for (int q = 0; q < 4; ++q) {               // which of 32 keys the row sees, as bits
+                        const int from = key0 + 32 * q, d = from - prefix;
+                        uint32_t there = piece_shift >= 5 ? (loaded >> ((32 * q) >> piece_shift) & 1u ? 0xffffffffu : 0u)
+                                                          : ((loaded >> (2 * q) & 1u ? 0xffffu : 0u) | (loaded >> (2 * q + 1) & 1u ? 0xffff0000u : 0u));
+                        there &= below(w.length - from);
+                        const uint32_t drafts = d >= 64 || d <= -32 ? 0u : (d >= 0 ? (uint32_t)(sees >> d) : (uint32_t)sees << -d);
+                        const uint32_t seen = row_on ? there & (below(-d) | drafts) : 0u;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const int key = key0 + 32 * q + e, d = key - prefix;
-                            const bool seen = key < w.length && row_on && (loaded >> ((32 * q + e) >> piece_shift) & 1u) && (d < 0 || (sees >> (d & 63) & 1ull));
-                            if (!seen) x[q][e] = 0xff800000u;
-                        }
+                        for (int e = 0; e < 32; ++e)
+                            if (!(seen >> e & 1u)) x[q][e] = 0xff800000u;
+                    }
                 }
                 float top[4];
 #pragma unroll
@@ -337,26 +348,20 @@ cached_wide_kernel(const CachedParams p, const __grid_constant__ CUtensorMap map
             constexpr int kHalf = kDim / 2;
             float mine = 1.0f, theirs = 0.0f;
             const bool whole = w.tile == 0 && n == w.tiles;
+            bool any = false;
+            const int64_t part = (int64_t)blockIdx.x * 2 + (w.tile == 0 ? 1 : 0);
+            uint8_t* out = static_cast<uint8_t*>(p.o) +
+                (((int64_t)w.b * p.drafts + draft) * (p.kv_heads * p.group) + head * p.group + row - draft * p.group) * kDim * 2;
             if (s == 1) bars->ml[r] = make_float2(m, l);
+            // (short loops: this code runs once per segment, and unrolled its instructions took longer to fetch than to run)
 #pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
-                uint32_t acc[kHalf / 32][32];
-#pragma unroll
-                for (int q = 0; q < kHalf / 32; ++q) tc_ld_32x32b_x32(o_tmem + (uint32_t)(h * kHalf + 32 * q), acc[q]);
-                tc_wait_ld();
-                if (s == 1) {
-                    ok = wait_all(&bars->m_empty, ((uint32_t)m_no++ & 1u) ^ 1u, abort_flag, p.status);
-                    if (!ok) break;
-#pragma unroll
-                    for (int e = 0; e < kHalf; ++e) merge[e * kRowsTile + r] = __uint_as_float(acc[e / 32][e % 32]);
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bars->m_full);
-                    continue;
-                }
-                if (n > 1) {
-                    ok = wait_all(&bars->m_full, (uint32_t)m_no++ & 1u, abort_flag, p.status);
-                    if (!ok) break;
-                    if (h == 0) {
+            for (int h = 0; ok && h < 2; ++h) {
+                const bool joined = n > 1;
+                if (s == 1) ok = wait_all(&bars->m_empty, ((uint32_t)m_no++ & 1u) ^ 1u, abort_flag, p.status);
+                else if (joined) ok = wait_all(&bars->m_full, (uint32_t)m_no++ & 1u, abort_flag, p.status);
+                if (!ok) break;
+                if (s == 0 && h == 0) {
+                    if (joined) {
                         const float2 other = bars->ml[r];
                         const float higher = fmaxf(m, other.x), ref = higher == -INFINITY ? 0.0f : higher;
                         mine = attn_exp2(m - ref);
@@ -364,37 +369,48 @@ cached_wide_kernel(const CachedParams p, const __grid_constant__ CUtensorMap map
                         m = higher;
                         l = l * mine + other.y * theirs;
                     }
-                    // (a stream that saw nothing has weight 0, and may hold anything)
-#pragma unroll
-                    for (int e = 0; e < kHalf; ++e)
-                        acc[e / 32][e % 32] = __float_as_uint((mine == 0.0f ? 0.0f : __uint_as_float(acc[e / 32][e % 32]) * mine) +
-                                                              (theirs == 0.0f ? 0.0f : merge[e * kRowsTile + r] * theirs));
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bars->m_empty);
-                }
-                const bool any = row_on && l != 0.0f;               // false: the row sees nothing, and is zero whatever V holds
-                if (whole) {
-                    const float inv = any ? 1.0f / l : 0.0f;
-                    if (draft < p.drafts) {
-                        uint8_t* to = static_cast<uint8_t*>(p.o) +
-                            ((((int64_t)w.b * p.drafts + draft) * (p.kv_heads * p.group) + head * p.group + row - draft * p.group) * kDim + h * kHalf) * 2;
-#pragma unroll
-                        for (int q = 0; q < kHalf / 32; ++q) {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                if (!any) acc[q][e] = 0u;
-                            store_row32<kBf16>(to + 64 * q, acc[q], inv);
-                        }
-                    }
-                } else {
-                    const int64_t part = (int64_t)blockIdx.x * 2 + (w.tile == 0 ? 1 : 0);
-                    float* to = p.partial + part * (kRowsTile * kDim) + h * kHalf * kRowsTile + r;
-                    if (h == 0)
+                    any = row_on && l != 0.0f;                  // false: the row sees nothing, and is zero whatever V holds
+                    if (whole) {
+                        const float inv = any ? 1.0f / l : 0.0f;
+                        mine *= inv;
+                        theirs *= inv;
+                    } else {
                         reinterpret_cast<float2*>(p.partial + (int64_t)p.ctas * 2 * kRowsTile * kDim)[part * kRowsTile + r] =
                             any ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
-#pragma unroll
-                    for (int e = 0; e < kHalf; ++e) to[e * kRowsTile] = any ? __uint_as_float(acc[e / 32][e % 32]) : 0.0f;
+                    }
                 }
+#pragma unroll 1
+                for (int at = 0; at < kHalf; at += 16) {
+                    const int col = h * kHalf + at;
+                    uint32_t acc[16];
+                    tc_ld_32x32b_x16(o_tmem + (uint32_t)col, acc);
+                    tc_wait_ld();
+                    float* shared = merge + at * kRowsTile + r;
+                    if (s == 1) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) shared[e * kRowsTile] = __uint_as_float(acc[e]);
+                        continue;
+                    }
+                    float x[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {              // (a stream that saw nothing has weight 0, and may hold anything)
+                        x[e] = mine != 0.0f ? __uint_as_float(acc[e]) * mine : 0.0f;
+                        if (theirs != 0.0f) x[e] += shared[e * kRowsTile] * theirs;
+                        if (!any) x[e] = 0.0f;
+                    }
+                    if (whole) {
+                        uint32_t words[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) words[e] = pack2<kBf16>(x[2 * e], x[2 * e + 1]);
+                        if (draft < p.drafts) st_global_v8(out + col * 2, words);
+                    } else {
+                        float* to = p.partial + part * (kRowsTile * kDim) + col * kRowsTile + r;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) to[e * kRowsTile] = x[e];
+                    }
+                }
+                __syncwarp();
+                if (lane == 0 && joined) mbar_arrive(s == 1 ? &bars->m_full : &bars->m_empty);
             }
             if (!ok) break;
             t += n;
@@ -410,10 +426,11 @@ cached_wide_kernel(const CachedParams p, const __grid_constant__ CUtensorMap map
     }
 }
 
-// Joins the parts of one (sequence, key head, row tile), 16 columns: one row per thread.
+// Joins the parts of one (sequence, key head, row tile), kCols columns: one row per thread, many small CTAs whose loads
+// travel together.
 template <typename T, int kDim>
 __global__ void __launch_bounds__(kRowsTile) cached_wide_join_kernel(const CachedParams p) {
-    constexpr int kCols = 16;
+    constexpr int kCols = kJoinCols;
     const int lane = threadIdx.x & 31, r = threadIdx.x, hms = p.kv_heads * p.row_tiles;
     const int item = blockIdx.x / (kDim / kCols), col0 = (blockIdx.x - item * (kDim / kCols)) * kCols;
     const int b = item / hms, hm = item - b * hms, head = hm / p.row_tiles;
@@ -426,7 +443,7 @@ __global__ void __launch_bounds__(kRowsTile) cached_wide_join_kernel(const Cache
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (draft >= p.drafts || first == last) return;         // one CTA had all of it and wrote the output
     const float2* ml = reinterpret_cast<const float2*>(p.partial + (int64_t)p.ctas * 2 * kRowsTile * kDim);
-    constexpr int kBatch = 4;
+    constexpr int kBatch = 8;
     float sum[kCols], l = 0.0f, top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < kCols; ++e) sum[e] = 0.0f;
@@ -460,12 +477,11 @@ __global__ void __launch_bounds__(kRowsTile) cached_wide_join_kernel(const Cache
         }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T out[kCols];
+    __align__(8) T out[kCols];
 #pragma unroll
     for (int e = 0; e < kCols; ++e) out[e] = Scalar<T>::from_float(sum[e] * inv);
     T* to = static_cast<T*>(p.o) + (((int64_t)b * p.drafts + draft) * (p.kv_heads * p.group) + head * p.group + (row - draft * p.group)) * kDim + col0;
-    reinterpret_cast<uint4*>(to)[0] = reinterpret_cast<const uint4*>(out)[0];
-    reinterpret_cast<uint4*>(to)[1] = reinterpret_cast<const uint4*>(out)[1];
+    *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(out);
 }
 
 template <bool kBf16, int kDim>
@@ -477,7 +493,7 @@ int launch_wide(const CachedParams& p, const CUtensorMap& map_k, const CUtensorM
     // a scale of 0 stays a factor that keeps masked scores at -infinity
     kernel<<<p.ctas, kWideThreads, smem, stream>>>(p, map_k, map_v, p.scale_log2 < 0.0f, fmaxf(fabsf(p.scale_log2), 1e-37f));
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3((unsigned)(p.batch * p.kv_heads * p.row_tiles * (kDim / 16)));
+    config.gridDim = dim3((unsigned)(p.batch * p.kv_heads * p.row_tiles * (kDim / kJoinCols)));
     config.blockDim = dim3(kRowsTile);
     config.stream = stream;
     cudaLaunchAttribute overlap{};
@@ -501,7 +517,7 @@ int cached_wide(const CachedParams& given, int dtype, int64_t head_dim, const vo
     p.row_tiles = (p.drafts * p.group + kRowsTile - 1) / kRowsTile;
     p.ctas = sm_count();
     if (p.ctas <= 0) return BSA_ERR_LAUNCH;
-    if ((int64_t)p.row_tiles * p.kv_heads > (int64_t)INT32_MAX / p.batch / 8) return BSA_ERR_TOO_LARGE;
+    if ((int64_t)p.row_tiles * p.kv_heads > (int64_t)INT32_MAX / p.batch / 32) return BSA_ERR_TOO_LARGE;
     CUtensorMap map_k, map_v;
     const int64_t rows = (int64_t)p.pages * p.kv_heads * page;
     const int piece = (int)std::min<int64_t>(page, kRowsTile);
