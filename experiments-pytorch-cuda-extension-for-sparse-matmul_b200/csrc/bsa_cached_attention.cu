@@ -99,6 +99,32 @@ __device__ __forceinline__ uint32_t chunk_offset(int row, int chunk) {
     return (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
 }
 
+// Of 32 keys from key0 on, those (of `wanted`) whose block is in the layout, seen from block row `row`.  Whole blocks before
+// the drafts are one lookup per 16 keys; a draft stands behind the prefix and its ancestors.
+// (`at`: the row of the pattern; `tree`: the sequence's words, or null)
+__device__ __noinline__ uint32_t in_pattern(const uint8_t* at, int cols, int shift, const int64_t* tree, int key0, int prefix, uint32_t wanted) {
+    uint32_t bits = 0u;
+#pragma unroll 1
+    for (int k = 0; k < 32; ++k) {
+        const int key = key0 + k, draft = key - prefix;
+        if ((k & 15) == 0 && key + 16 <= prefix) {
+            const int block = key >> shift;
+            if (block < cols && at[block]) bits |= 0xffffu << k;
+            k += 15;
+            continue;
+        }
+        if (!(wanted >> k & 1u)) continue;
+        int place = key;
+        if (draft >= 0) {
+            const uint64_t w = tree ? (uint64_t)tree[draft] : ~0ull >> (63 - draft);
+            place = max(prefix, 0) + max(__popcll(w) - 1, 0);
+        }
+        const int block = place >> shift;
+        if (block < cols && at[block]) bits |= 1u << k;
+    }
+    return bits;
+}
+
 // T: type of q and o; kGroups: groups of 16 rows (1, 2 or 4).
 template <typename T, bool kE4m3, int kDim, int kGroups>
 __global__ void __launch_bounds__((kConsumers + 1) * 32, 2)
@@ -372,33 +398,34 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             const bool masked = tile_end > prefix || !all_loaded || p.pattern != nullptr;
             uint32_t keep[kNT];                             // per n-tile: which of this thread's two keys are really there
             if (masked) {
-                const int piece_shift = min(p.page_shift, 6);
+                // The step's 32 keys as bits: what is there, and what each of the two rows sees.  (Written out per element this
+                // was most of the kernel's code, and a short sequence, all of whose steps come here, waited for it to be fetched.)
+                const int shift = min(p.page_shift, 6), d = key0 - prefix;
+                uint32_t there = shift >= 5 ? (loaded >> (base >> shift) & 1u ? 0xffffffffu : 0u)
+                                            : ((loaded >> (base >> 4) & 1u ? 0xffffu : 0u) | (loaded >> ((base >> 4) + 1) & 1u ? 0xffff0000u : 0u));
+                there &= below(length - key0);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const uint32_t drafts = d >= 64 || d <= -32 ? 0u : (d >= 0 ? (uint32_t)(sees[r] >> d) : (uint32_t)sees[r] << -d);
+                    uint32_t seen = row_on[r] ? there & (below(-d) | drafts) : 0u;
+                    if (p.pattern)
+                        seen = row_block[r] < 0 || row_block[r] >= p.pattern_rows ? 0u :
+                            seen & in_pattern(p.pattern + (int64_t)row_block[r] * p.pattern_cols, p.pattern_cols, p.pattern_shift,
+                                              p.tree ? p.tree + (int64_t)b * p.drafts : nullptr, key0, prefix, seen);
+                    seen >>= 2 * c;
+#pragma unroll
+                    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (!(seen >> (8 * n + e) & 1u)) s[n][2 * r + e] = -INFINITY;
+                }
+                there >>= 2 * c;
 #pragma unroll
                 for (int n = 0; n < kNT; ++n) {
-                    keep[n] = 0;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int key = key0 + n * 8 + 2 * c + e, draft = key - prefix;
-                        const bool there = key < length && (loaded >> ((key & (kTileKeys - 1)) >> piece_shift) & 1u);
-                        if (there) keep[n] |= e ? 0xffff0000u : 0x0000ffffu;
-                        int key_block = -1;
-                        if (p.pattern && there) {
-                            int place = key;
-                            if (draft >= 0) {
-                                const uint64_t w = p.tree ? (uint64_t)p.tree[(int64_t)b * p.drafts + draft] : ~0ull >> (63 - draft);
-                                place = max(prefix, 0) + max(__popcll(w) - 1, 0);
-                            }
-                            key_block = place >> p.pattern_shift;
-                        }
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            bool seen = there && row_on[r] && (draft < 0 || (sees[r] >> draft & 1ull));
-                            if (p.pattern && seen)
-                                seen = row_block[r] < p.pattern_rows && key_block < p.pattern_cols &&
-                                       p.pattern[(int64_t)row_block[r] * p.pattern_cols + key_block] != 0;
-                            if (!seen) s[n][2 * r + e] = -INFINITY;
-                        }
-                        if (kE4m3 && !there) inv[n][e] = 0.0f;
+                    keep[n] = (there >> (8 * n) & 1u ? 0x0000ffffu : 0u) | (there >> (8 * n + 1) & 1u ? 0xffff0000u : 0u);
+                    if (kE4m3) {
+                        if (!(keep[n] & 1u)) inv[n][0] = 0.0f;
+                        if (!(keep[n] >> 16)) inv[n][1] = 0.0f;
                     }
                 }
             }

@@ -29,6 +29,9 @@ struct Share {
 
 namespace {
 
+// The lowest n bits.
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
+
 __device__ __forceinline__ int cached_length(const CachedParams& p, int b) {
     return min(max(p.lengths[b], 0), p.table_width << p.page_shift);
 }

@@ -40,9 +40,6 @@ struct __align__(16) WideBarriers {
 template <int kDim>
 constexpr int wide_smem() { return (1 + 2 * kWideStages) * (kDim / 64) * kPanelBytes + (int)sizeof(WideBarriers); }
 
-// The lowest n bits.
-__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
-
 // The share of a CTA, segment by segment: tiles of one (sequence, head, row tile).
 struct Walk {
     int64_t u, end;
