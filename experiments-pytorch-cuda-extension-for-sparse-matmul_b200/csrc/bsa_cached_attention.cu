@@ -39,10 +39,13 @@ constexpr int kBegin = 6;                       // what beginning and ending a (
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int64_t kWideRows = 32;               // query rows of a key head above which a 16-bit cache goes to the tcgen05 kernel
 
-template <int kStages>
+// Barriers go by the number of the tile, modulo kBars, and so belong to one stream of tiles each: a warp that skips the
+// other stream's tiles sees every phase of the barriers that it waits for.  (With a barrier per stage and an odd number of
+// stages it saw every second one, and could take a phase that had not begun for the one before it.)
+template <int kBars>
 struct __align__(8) CachedBarriers {
-    uint64_t full[kStages], empty[kStages];
-    uint32_t ok[kStages];           // bit i: page i of the stage's tile was loaded
+    uint64_t full[kBars], empty[kBars];
+    uint32_t ok[kBars];             // bit i: page i of the tile was loaded
     Share share;
     int abort_flag;
 };
@@ -81,13 +84,15 @@ struct CachedShape {
     static constexpr int kScaleBytes = kE4m3 ? 2 * kTileKeys * 4 : 0;
     static constexpr int kStageBytes = 2 * kSideBytes;
     static constexpr int kStages = kStageBytes >= 32768 ? 3 : (kStageBytes >= 16384 ? 5 : 8);
+    static constexpr int kStreams = kGroups == 1 ? 2 : 1;       // of tiles, see the kernel
+    static constexpr int kBars = kStages * (kStages % kStreams == 0 ? 1 : kStreams);
     // columns of O that the warps of a row group join at a time (the 8-bit layout stores pairs of 8-column tiles)
     static constexpr int kJoin = kE4m3 ? 64 : 32;
     static constexpr int kJoinFloats = kGroups == 4 ? 0 : kConsumers * 16 * (kJoin + 2);
     static constexpr int kRows = 16 * kGroups;
     static constexpr int kQueryBytes = kRows * (kDim * 2 + 4);                  // fragments, and a factor per row
     static constexpr int kKeyBytes = kE4m3 ? kConsumers * 32 * 16 : 0;          // what the warps make of their keys' scales
-    static constexpr int kSmem = kStages * (kStageBytes + kScaleBytes) + kKeyBytes + kQueryBytes + kJoinFloats * 4 + (int)sizeof(CachedBarriers<kStages>);
+    static constexpr int kSmem = kStages * (kStageBytes + kScaleBytes) + kKeyBytes + kQueryBytes + kJoinFloats * 4 + (int)sizeof(CachedBarriers<kBars>);
     static_assert(2 * (kSmem + 1024) <= 233472, "two CTAs per SM");
 };
 
@@ -130,14 +135,14 @@ template <typename T, bool kE4m3, int kDim, int kGroups>
 __global__ void __launch_bounds__((kConsumers + 1) * 32, 2)
 cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
     using S = CachedShape<kE4m3, kDim, kGroups>;
-    using Bars = CachedBarriers<S::kStages>;
+    using Bars = CachedBarriers<S::kBars>;
     constexpr bool kTBf16 = std::is_same_v<T, __nv_bfloat16>;
     constexpr bool kBf16 = !kE4m3 && kTBf16;                // type of the products
     constexpr int kRows = 16 * kGroups;
     constexpr int kSplit = kConsumers / kGroups;            // warps that share a row group
     // With one row group the warps work as two pairs on alternate tiles, 32 keys each: 16 keys per warp and tile leave
     // too few independent instructions between the tile's barriers.
-    constexpr int kStreams = kSplit == 4 ? 2 : 1;
+    constexpr int kStreams = S::kStreams;
     constexpr int kWarpKeys = kTileKeys * kStreams / kSplit;            // keys of a tile per warp
     constexpr int kStepKeys = 32;                           // keys of a step of the warp (registers)
     constexpr int kNT = kStepKeys / 8;
@@ -154,7 +159,7 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
         if (lane == 0) bars->share = mine;
     } else if (warp == kConsumers && lane == 0) {
         bars->abort_flag = 0;
-        for (int i = 0; i < S::kStages; ++i) {
+        for (int i = 0; i < S::kBars; ++i) {
             mbar_init(&bars->full[i], 1);
             mbar_init(&bars->empty[i], kConsumers / kStreams);
         }
@@ -164,8 +169,7 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
     const Share share = bars->share;
     int b = share.b, hm = share.hm, tile = share.tile;
     const int hms = p.kv_heads * p.row_tiles;
-    int stage = 0;
-    uint32_t phase = 0;
+    uint32_t turn = 0;                                      // tiles so far
 
     if (warp == kConsumers) {                               // ---- producer
         // One lane per copy of a tile, so that all leave with one instruction: pages (at most 4) x sides x panels of the
@@ -211,22 +215,26 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             }
             if (u < share.end) look();
             const uint32_t loaded = __ballot_sync(0xffffffffu, ok) & 15u;
-            dead = !mbar_wait(&bars->empty[stage], phase ^ 1, &bars->abort_flag, p.status);
+            const uint32_t stage = turn % S::kStages, bar = turn % S::kBars;
+            if (turn >= (uint32_t)S::kStages) {             // the stage's last tile has been read
+                const uint32_t last = turn - S::kStages;
+                dead = !mbar_wait(&bars->empty[last % S::kBars], last / S::kBars & 1u, &bars->abort_flag, p.status);
+            }
             if (dead) break;
             if (lane == 0) {
-                bars->ok[stage] = loaded;
-                mbar_expect_tx(&bars->full[stage], (uint32_t)(__popc(loaded) * piece * (2 * S::kRowBytes + (kE4m3 ? 8 : 0))));
+                bars->ok[bar] = loaded;
+                mbar_expect_tx(&bars->full[bar], (uint32_t)(__popc(loaded) * piece * (2 * S::kRowBytes + (kE4m3 ? 8 : 0))));
             }
             __syncwarp();
             if (ok && my_tile)
                 tma_load_3d(smem + stage * S::kStageBytes + my_side * S::kSideBytes + my_panel * (kTileKeys * S::kPanelBytes) +
-                            my_piece * piece * S::kPanelBytes, my_map, &bars->full[stage],
+                            my_piece * piece * S::kPanelBytes, my_map, &bars->full[bar],
                             my_panel * (S::kPanelBytes / (kE4m3 ? 1 : 2)), row, 0);
             if (ok && my_scale)
                 bulk_load_1d(scale_smem + stage * S::kScaleBytes + my_side * (kTileKeys * 4) + my_piece * piece * 4,
-                             p.scales[my_side] + row, (uint32_t)(piece * 4), &bars->full[stage]);
+                             p.scales[my_side] + row, (uint32_t)(piece * 4), &bars->full[bar]);
             __syncwarp();
-            if (++stage == S::kStages) { stage = 0; phase ^= 1; }
+            ++turn;
         }
         if (dead) let_copies_land();
         return;
@@ -235,7 +243,6 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
     // ---- consumers
     const int rg = warp / kSplit, part = warp % kSplit;     // row group; number among its warps
     const int stream = part % kStreams, first_key = part / kStreams * kWarpKeys;        // which tiles, which keys of them
-    uint32_t turn = 0;                                      // tiles so far
     const int g = lane >> 2, c = lane & 3;
     // addresses of this lane's ldmatrix rows inside 8 keys (K) and 16 keys (V)
     uint32_t k_lane[S::kRowBytes / 64];
@@ -326,13 +333,11 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
         for (int i = 0; i < todo; ++i, ++tile, ++turn) {
-            if (kStreams == 2 && (int)(turn & 1) != stream) {
-                if (++stage == S::kStages) { stage = 0; phase ^= 1; }
-                continue;
-            }
-            if (!dead) dead = !mbar_wait(&bars->full[stage], phase, &bars->abort_flag, p.status);
+            if (kStreams == 2 && (int)(turn & 1) != stream) continue;
+            const uint32_t stage = turn % S::kStages, bar = turn % S::kBars;
+            if (!dead) dead = !mbar_wait(&bars->full[bar], turn / S::kBars & 1u, &bars->abort_flag, p.status);
             const uint32_t k_base = smem_u32(smem) + stage * S::kStageBytes, v_base = k_base + S::kSideBytes;
-            const uint32_t loaded = bars->ok[stage];
+            const uint32_t loaded = bars->ok[bar];
 #pragma unroll 1
             for (int base = first_key; base < first_key + kWarpKeys; base += kStepKeys) {
             const int key0 = tile * kTileKeys + base;
@@ -496,8 +501,7 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->empty[stage]);
-            if (++stage == S::kStages) { stage = 0; phase ^= 1; }
+            if (lane == 0) mbar_arrive(&bars->empty[bar]);
         }
         // the quad's four partial sums of a row
 #pragma unroll

@@ -412,6 +412,9 @@ ATTENTION = [
     (128, 16, 1, 16, 3, [1, 2, 3, 127, 128, 129, 255, 256, 257, 0, 700], None, False),
     (64, 64, 8, 8, 8, [50, 3000, 8, 0, 131] * 9, [8, 3, 8, 0, 1] * 9, True),
     (128, 128, 4, 5, 60, [60, 61, 9000], None, True),
+    # many tiles per share: every stage of the ring is used again and again, by both streams of tiles
+    (128, 64, 4, 8, 1, [4000] * 8, None, False),
+    (64, 16, 2, 4, 2, [20000, 5, 9000], None, False),
 ]
 
 
