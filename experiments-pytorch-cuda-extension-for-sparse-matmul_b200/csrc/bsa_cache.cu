@@ -9,10 +9,11 @@
 //     Reading gives round16(code * scale): one rounding to 16 bits, of the product held in fp32.
 //
 // 16 elements of a token's head per thread: head_dim / 16 neighbouring lanes hold a row, whose maximum is that of packed
-// 16-bit magnitudes and two or three shuffles; a lane group takes one token and up to four of its heads, keys and values,
-// so a token's place is computed once and up to eight 32-byte loads are in flight.  Both kernels move each byte once:
-// bound by DRAM at prompt sizes, by the launch at decoding sizes.  (One row and side per lane group of 16 lanes spent
-// its time on addresses: 36 us for 16,000 tokens of 8 x 128.)
+// 16-bit magnitudes and two or three shuffles; a lane group takes one token and two of its heads, keys and values,
+// so a token's place is computed once and four 32-byte loads are in flight.  Both kernels move each byte once:
+// bound by DRAM at prompt sizes (16,000 tokens of 8 heads x 128 into e4m3: 20.4 us, 4.9 TB/s; read back: 20.6 us), by the
+// launch at decoding sizes (1.7 us for 512 rows in a graph, 5 us as a call).  (One row and side per group of 16 lanes spent
+// its time on addresses: 36 us; four heads per group on registers: 24 us.)
 #include <cuda_fp8.h>
 
 #include "bsa_common.cuh"
@@ -23,8 +24,10 @@ namespace {
 constexpr float kE4m3Max = 448.0f;
 constexpr float kAmaxFloor = 0x1p-100f;
 
-constexpr int kWideHeads = 2;
-constexpr int64_t kNarrowRows = 4096;          // tokens x heads below which a lane group takes one row
+constexpr int kWideHeads = 2;                   // at prompt sizes: 20.4 us, with 4: 24.4
+// Tokens x heads below which a lane group takes one row.  8-bit writes of 8 heads x 128, one row / two heads of both sides, in
+// a replayed graph: 512 rows 1.7 / 2.4 us, 4096 2.2 / 2.8, 8192 2.6 / 2.9, 16384 3.4 / 3.5, 32768 5.0 / 4.8, 128000 16.8 / 15.0.
+constexpr int64_t kNarrowRows = 16384;
 
 struct CacheParams {
     const void* src[2];             // write: the tokens' keys / values; read: the cache's
@@ -197,7 +200,7 @@ int launch_shape(bool write, const CacheParams& p, cudaStream_t stream) {
 }
 template <typename T, bool kE4m3, int kDim>
 int launch(bool write, const CacheParams& p, cudaStream_t stream) {
-    // few rows: one load per thread is the shortest way; many: eight in flight
+    // few rows: one load per thread is the shortest way; many: four in flight
     const int64_t rows = (int64_t)p.tokens * p.heads;
     return rows < kNarrowRows ? launch_shape<T, kE4m3, kDim, 1, 1>(write, p, stream)
                               : launch_shape<T, kE4m3, kDim, kWideHeads, 2>(write, p, stream);

@@ -21,6 +21,10 @@
 //   warp 9           MMA issuer: S0 S1 | PV0 S0' PV1 S1' | ..; each PV in two parts, the first while the second half of P is made
 // The last K / V tile of a sequence may hold rows of the next one; its V rows are zeroed before use (see zero_rows).
 // All waits are bounded.
+//
+// 16,127 rows of 8 sequences, 16 / 4 heads x 128, bf16: 227 us, 930 TFLOP/s (194 us replayed on the same inputs).  A pair of tiles takes
+// 3100 cycles where the tensor pipe needs 2048: the chain of one tile (waiting for its MMAs 1130 cycles, 400 until its maximum,
+// 1330 of exponentials) is half hidden behind the other's.
 #include <type_traits>
 
 #include "bsa_packed_common.cuh"
@@ -30,7 +34,6 @@ namespace {
 
 constexpr int kFwdStages = 4;
 constexpr int kFwdThreads = 320;
-constexpr int kPoly = 0;                        // every kPoly-th pair of exponentials goes to the FMA pipe
 
 struct PackedParams {
     void* o;
@@ -368,15 +371,10 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
                     for (int i = 2 * half; i < 2 * half + 2; ++i)
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
-                            const uint64_t y = f2_fma(f2_pack(__uint_as_float(x[i][e]), __uint_as_float(x[i][e + 1])), c2, ref2);
                             float a, b;
-                            if (kPoly > 0 && (e / 2) % (kPoly > 0 ? kPoly : 1) == 1 && !masked) {
-                                exp2_pair(y, a, b);
-                            } else {
-                                f2_unpack(y, a, b);
-                                a = attn_exp2(a);
-                                b = attn_exp2(b);
-                            }
+                            f2_unpack(f2_fma(f2_of(x[i][e], x[i][e + 1]), c2, ref2), a, b);
+                            a = attn_exp2(a);
+                            b = attn_exp2(b);
                             sum[(e / 2) & 1] = f2_add(sum[(e / 2) & 1], f2_pack(a, b));
                             x[half][(i & 1) * 16 + e / 2] = pack2<kBf16>(a, b);
                         }

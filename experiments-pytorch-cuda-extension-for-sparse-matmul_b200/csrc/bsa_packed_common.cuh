@@ -155,32 +155,6 @@ __device__ __forceinline__ void tc_st_32x32b_x8(uint32_t taddr, const uint32_t (
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 
-__device__ __forceinline__ uint64_t f2_sub(uint64_t a, uint64_t b) { return f2_add(a, b ^ 0x8000000080000000ull); }
-__device__ __forceinline__ float fmax_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-// 2^x of two values on the FMA pipe: x = n + f, n the nearest integer (by adding 1.5 * 2^23, which leaves n in the low
-// bits), 2^f by its polynomial of degree 4 with the smallest largest relative error on [-1/2, 1/2] (2.6e-6, found by
-// Remez exchange), 2^n from the exponent bits.  x is kept above -125 (2^-125 in place of anything smaller); NaN stays.
-// The MUFU units give 16 exponentials a cycle and SM, this form takes a quarter of them off their hands.
-__device__ __forceinline__ void exp2_pair(uint64_t x, float& a, float& b) {
-    float x0, x1, t0, t1;
-    f2_unpack(x, x0, x1);
-    x = f2_pack(fmax_nan(x0, -125.0f), fmax_nan(x1, -125.0f));
-    const uint64_t magic = f2_pack(12582912.0f, 12582912.0f);
-    const uint64_t t = f2_add(x, magic);
-    const uint64_t f = f2_sub(x, f2_sub(t, magic));
-    uint64_t y = f2_fma(f2_pack(0.009570102207362652f, 0.009570102207362652f), f, f2_pack(0.05591785907745361f, 0.05591785907745361f));
-    y = f2_fma(y, f, f2_pack(0.240247443318367f, 0.240247443318367f));
-    y = f2_fma(y, f, f2_pack(0.6931217908859253f, 0.6931217908859253f));
-    y = f2_fma(y, f, f2_pack(0.9999992847442627f, 0.9999992847442627f));
-    f2_unpack(t, t0, t1);
-    const uint64_t scale = f2_pack(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u));
-    f2_unpack(f2_mul(y, scale), a, b);
-}
-
 __device__ __forceinline__ uint64_t f2_of(uint32_t lo, uint32_t hi) { return f2_pack(__uint_as_float(lo), __uint_as_float(hi)); }
 
 // Zeroes rows [from, 128) of a tile in shared memory (all lanes of a warp), for the tensor cores to read: what TMA
@@ -272,7 +246,7 @@ bool bind_device() {
     return false;
 }
 
-// Argument checks of both directions; `tensors`: pointers that must be there and 16-byte aligned.
+// Checks of the types and sizes of both directions.
 int check_packed(int dtype, int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim) {
     if (dtype != BSA_DTYPE_F16 && dtype != BSA_DTYPE_BF16) return BSA_ERR_BAD_DTYPE;
     if (dim != 64 && dim != 128) return BSA_ERR_BAD_SHAPE;

@@ -14,12 +14,15 @@
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/graph_task.h>
 
 #include <map>
 #include <mutex>
 #include <string>
 #include <tuple>
+#include <unordered_set>
 #include <vector>
 
 #include "bsa.h"
@@ -625,6 +628,36 @@ void check_device_status(int64_t device_index) {
                  "check_device_status");
 }
 
+// A backward pass under capture must not reach nodes that belong to the default stream, which cannot join a capture: those
+// of a graph recorded before it, or the accumulation nodes of leaves that such a graph, still alive, shares with it.  The
+// engine would make the default stream wait for the captured one and fail where an exception ends the process, so it is
+// refused here, before anything is launched.
+void refuse_capture_with_default_stream() {
+    if (at::cuda::currentStreamCaptureStatus() == at::cuda::CaptureStatus::None) return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    const auto* wanted = torch::autograd::get_current_graph_task_exec_info();
+    std::vector<torch::autograd::Node*> open{node.get()};
+    std::unordered_set<torch::autograd::Node*> seen;
+    while (!open.empty()) {
+        auto* const at = open.back();
+        open.pop_back();
+        for (const auto& edge : at->next_edges()) {
+            auto* const next = edge.function.get();
+            if (!next || !seen.insert(next).second) continue;
+            if (wanted && !wanted->empty()) {                // autograd.grad: only what it has to pass
+                const auto it = wanted->find(next);
+                if (it == wanted->end() || !it->second.should_execute()) continue;
+            }
+            const auto stream = next->stream();
+            TORCH_CHECK(!stream || *stream != at::cuda::getDefaultCUDAStream(stream->device_index()).unwrap(),
+                        "packed_attention: this backward pass is being captured, but a graph that was recorded on the default "
+                        "stream still holds some of its leaves or nodes; drop it (its outputs and losses) before the capture");
+            open.push_back(next);
+        }
+    }
+}
+
 // packed_attention as an autograd op.  It lives here and not in Python because a small step (a few hundred rows) is bound by
 // the host: the backward then runs without the interpreter.  `check`: read the device status after each pass.
 class PackedAttention : public torch::autograd::Function<PackedAttention> {
@@ -640,6 +673,7 @@ public:
     }
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "packed_attention has no second derivative (create_graph=True)");
+        refuse_capture_with_default_stream();
         const auto saved = ctx->get_saved_variables();
         auto [dq, dk, dv] = packed_attention_backward(saved[0], saved[1], saved[2], saved[3], saved[4], grads[0], saved[5], saved[6],
                                                       ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool());

@@ -199,6 +199,36 @@ def test_write_then_read(dtype, store, tokens, heads, dim, page):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("store", ["same", "e4m3"])
+@pytest.mark.parametrize("heads,dim", [(1, 64), (5, 64), (3, 128)])
+def test_many_rows_and_odd_heads(store, heads, dim):
+    """The same rows at once (two heads of both sides per lane group) and in small calls (one row): the same bits."""
+    from sparse import cache_read, cache_write, make_cache
+    tokens, page, dtype = 16384 // heads + 77, 64, torch.float16
+    pages = -(-tokens // page) + 1
+    slots = torch.randperm(pages * page)[:tokens].cuda()
+    slots[5::11] = -1
+    k, v = (_normal((tokens, heads, dim), 8 + i, dtype, spread=3.0).cuda() for i in range(2))
+    caches = [make_cache(pages, page, heads, dim, E4M3 if store == "e4m3" else dtype) for _ in range(2)]
+    for cache in caches:
+        for t in cache:
+            if t is not None:
+                (t.view(torch.uint8) if t.dtype == E4M3 else t).fill_(3)
+    cache_write(k, v, slots, *caches[0])
+    for i in range(0, tokens, 1000):
+        cache_write(k[i:i + 1000], v[i:i + 1000], slots[i:i + 1000], *caches[1])
+    for a, b in zip(*caches):
+        if a is not None:
+            assert _same(*((x.view(torch.uint8) if x.dtype == E4M3 else x) for x in (a, b)))
+    whole = cache_read(slots, *caches[0], dtype=dtype)
+    parts = [cache_read(slots[i:i + 1000], *caches[0], dtype=dtype) for i in range(0, tokens, 1000)]
+    for side in range(2):
+        assert _same(whole[side], torch.cat([p[side] for p in parts]))
+        assert (whole[side][slots < 0] == 0).all()
+    _status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", ["same", "e4m3"])
 def test_write_takes_strided_and_misaligned_tokens(store):
     from sparse import cache_read, cache_write, make_cache
     dtype, tokens, heads, dim = torch.bfloat16, 21, 4, 64

@@ -93,7 +93,7 @@ def _reference(q, k, v, do, lengths, scale, causal):
             # fp32: a score is off by (d + 8) steps of its sum of magnitudes, relative in the weight and again in the row's
             # sum; 2^-20 for the exponential; P rounded once to 16 bits (relative u; in fp16 also 2^-25 of 2^8 at most,
             # the running maximum being kept within 2^8)
-            off = 2 * (d + 8) * 2.0 ** -24 * ((qh.abs() @ kh.abs().T) * abs(scale) * seen).amax(-1, keepdim=True) + 2.0 ** -18
+            off = 2 * (d + 8) * 2.0 ** -24 * ((qh.abs() @ kh.abs().T) * abs(scale) * seen).amax(-1, keepdim=True) + 2.0 ** -20
             p_max = p.amax(-1, keepdim=True)
             floor = tiny * p_max                            # an unnormalised weight 1 stands for at least p_max / 2^8 .. p_max
             e_p = (u + off) * p + floor * seen              # error of the weights that multiply V, per element
@@ -382,6 +382,47 @@ def test_training_step_in_a_graph_follows_its_offsets():
             t.fill_(7)
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(captured, want))
+    _status()
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore:The AccumulateGrad node's stream does not match")
+@pytest.mark.parametrize("through", ["grad", "backward", "a layer before"])
+def test_capture_beside_a_living_eager_graph_is_refused(through):
+    """The accumulation nodes of the leaves belong to the default stream as long as the eager graph lives."""
+    from sparse import packed_attention
+    q, k, v, do, offsets = _inputs([100, 28], 0, 4, 2, 64, torch.bfloat16, 21)
+    q, k, v = (t.cuda().requires_grad_() for t in (q, k, v))
+    do, offsets = do.cuda(), offsets.cuda()
+
+    def forward():
+        return packed_attention(*((t * 2 for t in (q, k, v)) if through == "a layer before" else (q, k, v)), offsets, 0.1)
+
+    def backward(out):
+        if through == "grad":
+            return torch.autograd.grad(out, (q, k, v), do)
+        for t in (q, k, v):
+            t.grad = None
+        out.backward(do)
+        return q.grad, k.grad, v.grad
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = [t.clone() for t in backward(forward())]
+    torch.cuda.current_stream().wait_stream(side)
+    eager = forward()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = forward()
+        with pytest.raises(RuntimeError, match="recorded on the default"):
+            backward(out)
+    del out, eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = backward(forward())
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(captured, want))
     _status()
 
 
