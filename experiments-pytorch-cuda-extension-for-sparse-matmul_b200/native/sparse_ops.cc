@@ -15,6 +15,7 @@
 
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/graph_task.h>
 
@@ -64,7 +65,24 @@ torch::Tensor workspace_for(const torch::Device& device) {
     std::lock_guard<std::mutex> lock(mutex);
     auto it = cache.find(device.index());
     if (it == cache.end()) {
-        auto ws = torch::zeros({BSA_WORKSPACE_BYTES}, torch::TensorOptions().dtype(torch::kUInt8).device(device));
+        const auto options = torch::TensorOptions().dtype(torch::kUInt8).device(device);
+        c10::cuda::CUDAGuard guard(device);
+        torch::Tensor ws;
+        if (at::cuda::currentStreamCaptureStatus() == at::cuda::CaptureStatus::None) {
+            ws = torch::zeros({BSA_WORKSPACE_BYTES}, options);
+        } else {
+            // A first call under capture: zeros there would be filled at each replay and not before.  Memory outside the
+            // graph's pool, cleared now and kept as long as the process.
+            c10::cuda::CUDAStreamCaptureModeGuard relaxed{cudaStreamCaptureModeRelaxed};
+            void* memory = nullptr;
+            cudaStream_t stream = nullptr;
+            C10_CUDA_CHECK(cudaMalloc(&memory, BSA_WORKSPACE_BYTES));
+            C10_CUDA_CHECK(cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking));
+            C10_CUDA_CHECK(cudaMemsetAsync(memory, 0, BSA_WORKSPACE_BYTES, stream));
+            C10_CUDA_CHECK(cudaStreamSynchronize(stream));
+            C10_CUDA_CHECK(cudaStreamDestroy(stream));
+            ws = torch::from_blob(memory, {BSA_WORKSPACE_BYTES}, options);
+        }
         it = cache.emplace(device.index(), ws).first;
     }
     return it->second;
