@@ -47,10 +47,20 @@ def tree_words(parents: Sequence[Sequence[int]], device=None) -> torch.Tensor:
 
 
 def _pattern(layout: SparseLayout, device: torch.device) -> torch.Tensor:
-    """The layout's block flags as the kernel reads them (made once per layout object and device)."""
+    """The layout's block flags as the kernel reads them, made once per layout object and device: the first call waits for
+    them, since later ones may come on other streams.  Under capture they are made in the graph, at each replay, and not
+    kept."""
     held = getattr(layout, "_cached_pattern", None)
     if held is None or held.device != device:
+        capturing = device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+        if capturing and layout.pattern.device != device:
+            raise RuntimeError("cached_attention: the layout's pattern is on another device; call once with this layout before "
+                               "the capture")
         held = (layout.pattern != 0).to(device=device, dtype=torch.uint8).contiguous()
+        if capturing:
+            return held
+        if held.is_cuda:
+            torch.cuda.current_stream(device).synchronize()
         layout._cached_pattern = held
     return held
 

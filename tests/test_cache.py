@@ -3,6 +3,9 @@ types and masks where they can go wrong, their refusals, and a run of them toget
 import ctypes
 import math
 import os
+import subprocess
+import sys
+import textwrap
 
 import pytest
 import torch
@@ -610,3 +613,46 @@ def test_offsets_behind_32_bits():
     want = torch.einsum("hn,nhd->hd", p, v.double())
     # two roundings to fp16 of values up to max |v|
     assert ((got[0, 0].double() - want).abs() <= 3 * 2.0 ** -11 * v.abs().max()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("restricted", [False, True])
+def test_first_call_of_a_process_under_capture(restricted):
+    """What a first call sets up (the workspace, the layout's flags) does not depend on a replay."""
+    script = textwrap.dedent("""
+        import torch
+        from sparse import SparseLayout, cache_slots, cache_write, cached_attention, make_cache
+        from sparse.kernel import sparse_ops
+        torch.manual_seed(0)
+        layout = SparseLayout(torch.tensor([[1, 0], [1, 1]], device="cuda"), block=64) if RESTRICTED else None
+        k, v = (torch.randn(100, 2, 64, device="cuda", dtype=torch.float16) for _ in range(2))
+        q = torch.randn(1, 1, 4, 64, device="cuda", dtype=torch.float16)
+        cache = make_cache(8, 16, 2, 64, torch.float16, "cuda")
+        table = torch.arange(8, device="cuda", dtype=torch.int32)[None]
+        lengths = torch.full((1,), 100, device="cuda", dtype=torch.int32)
+        slots = cache_slots(table, torch.zeros(100, dtype=torch.int64, device="cuda"), torch.arange(100, device="cuda"), 16)
+        # blocks of memory to be handed out again, holding anything but zeros
+        dirt = [torch.full((n,), 255, dtype=torch.uint8, device="cuda") for n in (4, 64, 512, 4096) * 8]
+        del dirt
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            cache_write(k, v, slots, *cache)
+            captured = cached_attention(q, *cache, table, lengths, scale=0.125, layout=layout)
+        sparse_ops.check_device_status(0)              # nothing has run
+        cache_write(k, v, slots, *cache)
+        eager = cached_attention(q, *cache, table, lengths, scale=0.125, layout=layout)
+        sparse_ops.check_device_status(0)
+        captured.zero_()
+        graph.replay()
+        assert torch.equal(captured, eager)
+        table.fill_(8)                                 # pages that are not the cache's: reported by a replay
+        graph.replay()
+        try:
+            sparse_ops.check_device_status(0)
+        except RuntimeError:
+            print("first call under capture: ok")
+    """).replace("RESTRICTED", str(restricted))
+    done = subprocess.run([sys.executable, "-c", script], env=dict(os.environ, PYTHONPATH=PKG), capture_output=True,
+                          text=True, timeout=300)
+    assert done.returncode == 0 and "first call under capture: ok" in done.stdout, done.stderr[-2000:]
