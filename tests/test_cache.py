@@ -473,6 +473,17 @@ def test_cached_attention_scales_of_all_sizes(store):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+@pytest.mark.parametrize("store,group,drafts", [("same", 2, 2), ("e4m3", 2, 2), ("same", 8, 12)])
+def test_cached_attention_negative_and_zero_scale(store, group, drafts, scale):
+    """The largest score is the smallest product, or all are equal; what is masked stays out (0 times an infinity)."""
+    case = _Case(torch.bfloat16, store, 64, 32, 2, group, drafts, [300, 40, 1], counts=[drafts, 1, 1], seed=31)
+    case.scale = scale
+    _check(case.call(), case.reference())
+    _status()
+
+
+@pytest.mark.gpu
 def test_cached_attention_tiny_and_huge_queries():
     """bf16 queries outside fp16's range over an 8-bit cache."""
     case = _Case(torch.bfloat16, "e4m3", 64, 16, 1, 4, 1, [90], seed=8)
