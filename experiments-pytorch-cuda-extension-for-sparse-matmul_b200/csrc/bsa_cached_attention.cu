@@ -26,9 +26,9 @@
 //
 // P is rounded to the products' 16-bit type (half a step: relative 2^-8 in bf16, 2^-11 in fp16), l, m and O are fp32.
 //
-// 32 sequences of 1 to 8192 tokens, 8 heads x 128, e4m3 (94 MB): 32.8 us, 2.9 TB/s; bound by the latency of a warp's step of 32
-// keys (2100 cycles with 2 consumer warps per scheduler) and what begins a share (2,800 cycles) and ends it (2,200 to 5,400).  One token over 391: 10.3 us a call, 8.8 in a
-// graph.
+// 32 sequences of 1 to 8192 tokens, 8 heads x 128, e4m3 (94 MB): 32.9 us, 2.9 TB/s; bound by the latency of a warp's
+// step of 32 keys (2100 cycles with 2 consumer warps per scheduler) and what begins a share (2,800 cycles) and ends it
+// (2,200 to 5,400).  One token over 391: 10.3 us a call, 8.8 in a graph.
 #include <algorithm>
 #include <type_traits>
 

@@ -2,8 +2,8 @@
 // bsa_cached_attention.cu, on tcgen05.
 //
 // With that many rows the m16n8k16 kernel is bound by its own instructions (24 drafts x 4 heads over 46,000 tokens: 70 us,
-// of which the cache's 94 MB take 14; here 40.8 us).  Here the rows of a key head, up to 128, are one M = 128 tile; keys go in tiles of
-// 128, and two streams of tiles, even and odd, each with its own scores, maximum, sum and O in TMEM, take turns on the
+// of which the cache's 94 MB take 14; here 40.5 us).  Here the rows of a key head, up to 128, are one M = 128
+// tile; keys go in tiles of 128, and two streams of tiles, even and odd, each with its own scores, maximum, sum and O in TMEM, take turns on the
 // tensor cores and in the softmax, as the two query tiles of the packed forward do; at the end the second hands its O to
 // the first.  The units (tiles of a sequence, key head and row tile) are shared out evenly over the SMs as in the other
 // kernel; a CTA that holds all of a sequence's tiles writes the output, the others leave (O, m, l) in fp32, columns by

@@ -22,9 +22,9 @@
 // The last K / V tile of a sequence may hold rows of the next one; its V rows are zeroed before use (see zero_rows).
 // All waits are bounded.
 //
-// 16,127 rows of 8 sequences, 16 / 4 heads x 128, bf16: 227 us, 930 TFLOP/s (194 us replayed on the same inputs).  A pair of tiles takes
-// 3100 cycles where the tensor pipe needs 2048: the chain of one tile (waiting for its MMAs 1130 cycles, 400 until its maximum,
-// 1330 of exponentials) is half hidden behind the other's.
+// 16,127 rows of 8 sequences, 16 / 4 heads x 128, bf16: 219 to 227 us, 930 to 960 TFLOP/s (194 us replayed on the
+// same inputs).  A pair of tiles takes 3100 cycles where the tensor pipe needs 2048: the chain of one tile (waiting for
+// its MMAs 1130 cycles, 400 until its maximum, 1330 of exponentials) is half hidden behind the other's.
 #include <type_traits>
 
 #include "bsa_packed_common.cuh"

@@ -23,8 +23,8 @@
 //
 // P and dS are rounded to the inputs' type before the accumulating products, everything else is fp32.
 //
-// 8,192 rows of 7 sequences, 16 / 4 heads x 128, bf16: statistics 24 us, keys 234, queries 177 (each alone, cold).  A tile takes 2400 cycles by
-// queries and 3500 by keys, bound by shared memory: a product of two operands there reads 128 bytes per cycle at the
+// 8,192 rows of 7 sequences, 16 / 4 heads x 128, bf16: statistics 24 us, keys 234, queries 177 (each alone,
+// cold).  A tile takes 2400 cycles by queries and 3500 by keys, bound by shared memory: a product of two operands there reads 128 bytes per cycle at the
 // tensor pipe's peak, all that an SM has, and the copies of the next tiles want 64 KB more.
 #include "bsa_packed_common.cuh"
 
