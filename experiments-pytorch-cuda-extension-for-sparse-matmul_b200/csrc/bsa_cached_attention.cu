@@ -18,13 +18,18 @@
 // at these row counts the tensor pipe idles either way, and a 128-row tcgen05 tile would be 7/8 padding.
 //
 // e4m3 caches.  Codes are exact in fp16, so the products run in fp16 on the codes themselves and the scales go where they
-// are cheap: the key's into the score, and the value's into the weight: with y_ij = log2(e) scale q_i k_j + log2 sv_j the
-// weights are P_ij = 2^(y_ij - m_i), m_i the running maximum of y (so P <= 2^8 whatever the scales are), O += P code,
-// l += P / sv_j, o = O / l.  bf16 queries are brought to fp16 by a power of two per row (exact but for values below
-// 2^-14 of the row's largest).  The 8-bit elements are paired by ldmatrix as 16-bit units, which permutes the
-// contraction axis of Q K^T (the query is loaded in the same order) and the columns of O (undone at the store).
+// are cheap: the key's into the score, the value's into the weight: P_ij = 2^(s_ij - m_i) as ever, l += P_ij, and
+// O += (P_ij sv_j / r) code.  r is a power of two per warp, raised lazily to the power of two under the largest finite |sv|
+// of the keys so far (as m is), so the weights stay below 2^8 x 16; O r is what goes out, so nothing outside the loop
+// knows of r.  l never sees a value's scale: a scale may be 0, negative, or 2^-109 (a row of zeros) beside 2^119.  A
+// weight below 2^-14 of r is rounded to steps of 2^-24 of it, so a row's error is relative to the largest stored values
+// of its sequence, as it is where fp16 holds the values themselves.  bf16 queries are brought to fp16 by a power of two
+// per row (exact but for values below 2^-14 of the row's largest).  The 8-bit elements are paired by ldmatrix as 16-bit
+// units, which permutes the contraction axis of Q K^T (the query is loaded in the same order) and the columns of O
+// (undone at the store).
 //
-// P is rounded to the products' 16-bit type (half a step: relative 2^-8 in bf16, 2^-11 in fp16), l, m and O are fp32.
+// The weights are rounded to the products' 16-bit type (half a step: relative 2^-8 in bf16, 2^-11 in fp16), l, m and O are
+// fp32.
 //
 // 32 sequences of 1 to 8192 tokens, 8 heads x 128, e4m3 (94 MB): 32.9 us, 2.9 TB/s; bound by the latency of a warp's
 // step of 32 keys (2100 cycles with 2 consumer warps per scheduler) and what begins a share (2,800 cycles) and ends it
@@ -42,6 +47,7 @@ constexpr int kConsumers = 4;                   // warps
 constexpr int kBegin = 6;                       // what beginning and ending a (sequence, head) costs a CTA, in tiles (batch of
                                                 // 32 of 1 to 8192 tokens: with 3 47.6 us, 5 37.4, 7 36.9, 10 38.5)
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint32_t kExponent = 1u << 23;        // one step of an fp32 number's exponent
 // Query rows of a key head above which a 16-bit cache goes to the tcgen05 kernel.  8 x 4000 tokens of 4 heads x 128: 32 rows
 // 26.7 us here, 30.0 us there; 40 rows 38.8 and 30.7, 128 rows 56.3 and 34.8.  16 x 300 tokens: 16.4 and 18.4; 20.5 and 18.4.
 constexpr int64_t kWideRows = 32;
@@ -98,7 +104,7 @@ struct CachedShape {
     static constexpr int kJoinFloats = kGroups == 4 ? 0 : kConsumers * 16 * (kJoin + 2);
     static constexpr int kRows = 16 * kGroups;
     static constexpr int kQueryBytes = kRows * (kDim * 2 + 4);                  // fragments, and a factor per row
-    static constexpr int kKeyBytes = kE4m3 ? kConsumers * 32 * 16 : 0;          // what the warps make of their keys' scales
+    static constexpr int kKeyBytes = kE4m3 ? kConsumers * 32 * 8 : 0;           // the scales of the warps' keys, the value's over r
     static constexpr int kSmem = kStages * (kStageBytes + kScaleBytes) + kKeyBytes + kQueryBytes + kJoinFloats * 4 + (int)sizeof(CachedBarriers<kBars>);
     static_assert(2 * (kSmem + 1024) <= 233472, "two CTAs per SM");
 };
@@ -155,7 +161,7 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
     constexpr int kNT = kStepKeys / 8;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* scale_smem = smem + S::kStages * S::kStageBytes;
-    float4* key_smem = reinterpret_cast<float4*>(scale_smem + S::kStages * S::kScaleBytes);
+    float* key_smem = reinterpret_cast<float*>(scale_smem + S::kStages * S::kScaleBytes);
     uint32_t* q_smem = reinterpret_cast<uint32_t*>(scale_smem + S::kStages * S::kScaleBytes + S::kKeyBytes);     // [row group][k step][lane][4]
     float* q_factor = reinterpret_cast<float*>(q_smem + kRows * kDim / 2);
     float* merge = q_factor + kRows;
@@ -338,6 +344,7 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
 #pragma unroll
             for (int e = 0; e < 4; ++e) out[i][e] = 0.0f;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        uint32_t r_bits = kExponent;                        // e4m3: r, a power of two from 2^-126 to 2^126; O is in units of it
 
         for (int i = 0; i < todo; ++i, ++tile, ++turn) {
             if (kStreams == 2 && (int)(turn & 1) != stream) continue;
@@ -347,7 +354,40 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             const uint32_t loaded = bars->ok[bar];
 #pragma unroll 1
             for (int base = first_key; base < first_key + kWarpKeys; base += kStepKeys) {
-            const int key0 = tile * kTileKeys + base;
+            const int key0 = tile * kTileKeys + base, tile_end = (tile + 1) * kTileKeys;
+            const bool all_loaded = loaded == (1u << (kTileKeys >> min(p.page_shift, 6))) - 1u;
+            const bool masked = tile_end > prefix || !all_loaded || p.pattern != nullptr;
+            // The step's 32 keys as bits: what is there, and below what each of the two rows sees.  (Written out per element this
+            // was most of the kernel's code, and a short sequence, all of whose steps are masked, waited for it to be fetched.)
+            uint32_t there = 0xffffffffu;
+            if (masked) {
+                const int shift = min(p.page_shift, 6);
+                there = shift >= 5 ? (loaded >> (base >> shift) & 1u ? 0xffffffffu : 0u)
+                                   : ((loaded >> (base >> 4) & 1u ? 0xffffu : 0u) | (loaded >> ((base >> 4) + 1) & 1u ? 0xffff0000u : 0u));
+                there &= below(length - key0);
+            }
+            // e4m3: a lane brings the scales of one key, the warp shares them (the key's, and the value's over r)
+            if (kE4m3) {
+                const float* scales = reinterpret_cast<const float*>(scale_smem + stage * S::kScaleBytes) + base + lane;
+                const float sv = there >> lane & 1u ? scales[kTileKeys] : 0.0f;
+                const uint32_t size = __float_as_uint(sv) & 0x7fffffffu;
+                const bool finite = size < 0x7f800000u;
+                if (__any_sync(0xffffffffu, finite && size >= r_bits + 4 * kExponent)) {
+                    const uint32_t top = min(__reduce_max_sync(0xffffffffu, finite ? size : 0u) & 0x7f800000u, 253 * kExponent);
+                    // 2^-(steps of the exponent), 0 where that is no normal number (of O nothing is left beside the new r)
+                    const uint32_t steps = top - r_bits;
+                    const float fall = __uint_as_float(127 * kExponent - min(steps, 127 * kExponent));
+                    r_bits = top;
+#pragma unroll
+                    for (int d = 0; d < kDim / 8; ++d)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) out[d][e] *= fall;
+                }
+                __syncwarp();                               // the last step's have been read
+                key_smem[warp * 64 + lane] = scales[0];
+                key_smem[warp * 64 + 32 + lane] = sv * __uint_as_float(254 * kExponent - r_bits);
+                __syncwarp();
+            }
             float s[kNT][4];
 #pragma unroll
             for (int n = 0; n < kNT; ++n)
@@ -381,41 +421,21 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
                     }
                 }
             }
-            // scores in units of log2; for e4m3 with the value's scale in the weight.  A lane makes what a key needs of its
-            // scales, the warp shares it: (key's scale, log2 of the value's, 1 / the value's).
-            float inv[kNT][2];
-            if (kE4m3) {
-                const float* scales = reinterpret_cast<const float*>(scale_smem + stage * S::kScaleBytes) + base + lane;
-                const float sv = scales[kTileKeys];
-                __syncwarp();                               // the last step's have been read
-                key_smem[warp * 32 + lane] = make_float4(scales[0], __log2f(sv), __fdividef(1.0f, sv), 0.0f);
-                __syncwarp();
-            }
+            // scores in units of log2
 #pragma unroll
             for (int n = 0; n < kNT; ++n) {
                 if (kE4m3) {
-                    const float4 k0 = key_smem[warp * 32 + n * 8 + 2 * c], k1 = key_smem[warp * 32 + n * 8 + 2 * c + 1];
-                    inv[n][0] = k0.z;
-                    inv[n][1] = k1.z;
+                    const float2 both = *reinterpret_cast<const float2*>(key_smem + warp * 64 + n * 8 + 2 * c);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[n][e] = fmaf(s[n][e] * ((e & 1) ? k1.x : k0.x), row_scale[e >> 1], (e & 1) ? k1.y : k0.y);
+                    for (int e = 0; e < 4; ++e) s[n][e] = s[n][e] * ((e & 1) ? both.y : both.x) * row_scale[e >> 1];
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[n][e] *= row_scale[e >> 1];
                 }
             }
-            const int tile_end = (tile + 1) * kTileKeys;
-            const bool all_loaded = loaded == (1u << (kTileKeys >> min(p.page_shift, 6))) - 1u;
-            const bool masked = tile_end > prefix || !all_loaded || p.pattern != nullptr;
             uint32_t keep[kNT];                             // per n-tile: which of this thread's two keys are really there
             if (masked) {
-                // The step's 32 keys as bits: what is there, and what each of the two rows sees.  (Written out per element this
-                // was most of the kernel's code, and a short sequence, all of whose steps come here, waited for it to be fetched.)
-                const int shift = min(p.page_shift, 6), d = key0 - prefix;
-                uint32_t there = shift >= 5 ? (loaded >> (base >> shift) & 1u ? 0xffffffffu : 0u)
-                                            : ((loaded >> (base >> 4) & 1u ? 0xffffu : 0u) | (loaded >> ((base >> 4) + 1) & 1u ? 0xffff0000u : 0u));
-                there &= below(length - key0);
+                const int d = key0 - prefix;
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const uint32_t drafts = d >= 64 || d <= -32 ? 0u : (d >= 0 ? (uint32_t)(sees[r] >> d) : (uint32_t)sees[r] << -d);
@@ -433,13 +453,8 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
                 }
                 there >>= 2 * c;
 #pragma unroll
-                for (int n = 0; n < kNT; ++n) {
+                for (int n = 0; n < kNT; ++n)
                     keep[n] = (there >> (8 * n) & 1u ? 0x0000ffffu : 0u) | (there >> (8 * n + 1) & 1u ? 0xffff0000u : 0u);
-                    if (kE4m3) {
-                        if (!(keep[n] & 1u)) inv[n][0] = 0.0f;
-                        if (!(keep[n] >> 16)) inv[n][1] = 0.0f;
-                    }
-                }
             }
             // The running maximum is raised only where a score exceeds it by more than 8 (units of log2): P stays below
             // 2^8, and O and l carry the same factor whatever it is.
@@ -468,12 +483,15 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
 #pragma unroll
             for (int r = 0; r < 2; ++r) ref[r] = m[r] == -INFINITY ? 0.0f : m[r];
 #pragma unroll
-            for (int n = 0; n < kNT; ++n)
+            for (int n = 0; n < kNT; ++n) {
+                const float2 over = kE4m3 ? *reinterpret_cast<const float2*>(key_smem + warp * 64 + 32 + n * 8 + 2 * c) : make_float2(1.0f, 1.0f);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     s[n][e] = attn_exp2(s[n][e] - ref[e >> 1]);
-                    l[e >> 1] += kE4m3 ? s[n][e] * inv[n][e & 1] : s[n][e];
+                    l[e >> 1] += s[n][e];
+                    if (kE4m3) s[n][e] *= (e & 1) ? over.y : over.x;
                 }
+            }
             // P V
 #pragma unroll
             for (int ks = 0; ks < kStepKeys / 16; ++ks) {
@@ -509,6 +527,12 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->empty[bar]);
+        }
+        if (kE4m3) {
+#pragma unroll
+            for (int d = 0; d < kDim / 8; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) out[d][e] *= __uint_as_float(r_bits);
         }
         // the quad's four partial sums of a row
 #pragma unroll

@@ -9,7 +9,8 @@ sizes of this package; head dimension 64 or 128).  It holds the tokens' own
     a = max(max_d |x_d|, 2^-100)    scale = a / 448    code_d = e4m3(x_d * (448 / a))
 
 so a stored value is ``code * scale``, within 2^-4 of itself or 2^-10 / 448 of the row's
-largest magnitude.  A row that holds an infinity or a NaN reads back as NaN.
+largest magnitude.  A row that holds an infinity or a NaN reads back as NaN.  Scales that another program made may be any
+finite number; those of a new cache are 0, so a place that was never written holds zeros.
 
 A token lives at ``slot = page_id * page + place``.  A sequence's pages are a
 row of a page table; ``cache_slots`` turns positions of sequences into slots.

@@ -285,7 +285,8 @@ int bsa_packed_backward(int dtype, const void* q, int64_t q_token_stride, int64_
  *   keys, values    [pages, heads, page, head_dim], contiguous, 32-byte aligned, as
  *                   the k and v that a read writes
  *   key_scales,
- *   value_scales    e4m3: float [pages, heads, page]; else ignored
+ *   value_scales    e4m3: float [pages, heads, page], any finite number where read
+ *                   (0 and negative ones too); else ignored
  * page 16, 32, 64 or 128; head_dim 64 or 128; pages * heads * page < 2^31.
  */
 int bsa_cache_write(int dtype, int store, const void* k, const void* v, int64_t k_token_stride,

@@ -667,3 +667,81 @@ def test_first_call_of_a_process_under_capture(restricted):
     done = subprocess.run([sys.executable, "-c", script], env=dict(os.environ, PYTHONPATH=PKG), capture_output=True,
                           text=True, timeout=300)
     assert done.returncode == 0 and "first call under capture: ok" in done.stdout, done.stderr[-2000:]
+
+
+# ------------------------------------------------------------------------------------------------ scales of every kind
+def _check_any_scale(case, pattern=None, block=1, **kw):
+    """As `_check`.  The weights P sv / r are rounded to fp16, r a power of two of at most the largest |sv| of a sequence
+    and head: below 2^-14 in steps of 2^-24, so that each of n keys is off by at most 2^-25 r 448, relative to a row sum
+    that is at least 1 / p_max.  (The bound of `_Case.reference` has the largest value of the column in place of 448 r,
+    which only holds where the scales are of one size.)"""
+    out, bound = case.reference(pattern, block)
+    for b, n in enumerate(case.lengths):
+        if n:
+            pages = case.table[b, :-(-n // case.page)].long()
+            top = case.value_scales[pages].double().abs().transpose(0, 1).flatten(1)[:, :n].amax(1).repeat_interleave(case.group)
+            bound[b] += n * 2.0 ** -25 * 448 * top[None, :, None]
+    _check(case.call(**kw), (out, bound))
+    _status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drafts,tree", [(1, False), (6, True), (22, True)])
+@pytest.mark.parametrize("kind", ["zero", "negative", "zeros beside huge ones", "all zero", "tiny"])
+def test_cached_attention_value_scales_of_any_kind(kind, drafts, tree):
+    """A stored value is code * scale whatever the scale is, and a key's weight does not depend on it: the softmax of a
+    place that was never written (scale 0) counts, that of a row of zeros (scale 2^-100 / 448) too."""
+    case = _Case(torch.bfloat16, "e4m3", 64, 16, 2, 3, drafts, [200, 50, 23], tree=tree, seed=41)
+    some = torch.rand(case.value_scales.shape, generator=torch.Generator().manual_seed(1)) < 0.4
+    if kind == "zero":
+        case.value_scales[some] = 0.0
+    elif kind == "negative":
+        case.value_scales[some] *= -1.0
+        case.key_scales[~some] *= -1.0
+    elif kind == "all zero":
+        case.value_scales[:] = 0.0
+    elif kind == "tiny":
+        case.value_scales *= 2.0 ** -90
+    else:
+        case.value_scales *= 2.0 ** 100
+        case.value_scales[some] = 2.0 ** -100 / 448
+        case.values.view(torch.uint8)[some] = 0
+    # (places that belong to no token keep a NaN scale)
+    case.value_scales[case.keys.float().isnan().any(-1)] = math.nan
+    case.k, case.v = (c.double() * s.double()[..., None] for c, s in ((case.keys, case.key_scales), (case.values, case.value_scales)))
+    _check_any_scale(case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drafts", [1, 4])
+def test_places_that_were_never_written_count_as_zeros(drafts):
+    """A length that covers skipped places and a padding sequence, over caches as `make_cache` gives them: the same weights
+    over 8 bits as over 16."""
+    from sparse import cache_slots, cache_write, cached_attention, make_cache
+    heads, group, dim, page, dtype = 2, 2, 64, 16, torch.float16
+    table = torch.arange(8, dtype=torch.int32).view(2, 4).cuda()
+    k, v = (_normal((50, heads, dim), i, dtype).cuda() for i in (1, 2))
+    q = _normal((2, drafts, heads * group, dim), 3, dtype).cuda()
+    slots = cache_slots(table, torch.zeros(50, dtype=torch.int64, device="cuda"), torch.arange(50, device="cuda"), page)
+    slots[3::7] = -1
+    lengths = torch.tensor([60, 20], dtype=torch.int32, device="cuda")      # 10 places behind the last token, and a sequence of none
+    for store in (dtype, E4M3):
+        cache = make_cache(8, page, heads, dim, store)
+        cache_write(k, v, slots, *cache)
+        got = cached_attention(q, *cache, table, lengths, scale=0.125).double()
+        every = cache_slots(table, torch.arange(2, device="cuda")[:, None], torch.arange(60, device="cuda"), page)
+        held = []
+        for side in range(2):
+            x = cache[side].double() if store == dtype else cache[side].double() * cache[2 + side].double()[..., None]
+            held.append(x[every // page, :, every % page].view(2, 60, heads, dim).repeat_interleave(group, 2))
+        s = torch.einsum("bihd,bjhd->bhij", q.double(), held[0]) * 0.125
+        at, n = torch.arange(60, device="cuda"), lengths[:, None, None]
+        seen = at <= n - drafts + torch.arange(drafts, device="cuda")[:, None]
+        want = torch.einsum("bhij,bjhd->bihd", torch.softmax(s.masked_fill(~seen[:, None], -math.inf), -1), held[1])
+        assert got.isfinite().all()
+        # the weights are rounded once (2^-11, or 2^-25 for each of 60 keys), so is the result; scores in fp32 (64 + 8 steps of
+        # their magnitudes, at most 64 * 4.5^2 / 8), twice, and 2^-20 for the exponential
+        off = 2 * 2.0 ** -11 + 60 * 2.0 ** -25 + 2 * 72 * 2.0 ** -24 * 162 + 2.0 ** -20
+        assert ((got - want).abs() <= off * held[1].abs().amax()).all()
+        assert (got[1] == 0).all()
+    _status()
