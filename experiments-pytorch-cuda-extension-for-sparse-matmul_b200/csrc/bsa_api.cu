@@ -66,7 +66,7 @@ extern "C" const char* bsa_status_string(int status) {
         case BSA_ERR_BAD_DTYPE: return "unsupported dtype";
         case BSA_ERR_BAD_SHAPE: return "bad shape: sizes must be positive and the sparse sides multiples of the block size";
         case BSA_ERR_BAD_BLOCK: return "block size must be 16, 32, 64 or 128";
-        case BSA_ERR_ALIGNMENT: return "device pointers must be 16-byte aligned";
+        case BSA_ERR_ALIGNMENT: return "device pointers must be 16-byte aligned (32-byte where the entry point says so)";
         case BSA_ERR_WORKSPACE: return "workspace missing or smaller than BSA_WORKSPACE_BYTES";
         case BSA_ERR_LAUNCH: return "CUDA launch failed";
         case BSA_ERR_DEVICE_TIMEOUT: return "a bounded wait inside a kernel ran out";

@@ -771,6 +771,8 @@ extern "C" int bsa_cached_attention(int dtype, int store, const void* q, int64_t
     if (q_batch_stride < 0 || q_draft_stride < 0 || q_head_stride < 0) return BSA_ERR_BAD_SHAPE;
     if (q_batch_stride % 8 || q_draft_stride % 8 || q_head_stride % 8) return BSA_ERR_ALIGNMENT;
     if (table_width > (int64_t)(INT32_MAX - 256) / page) return BSA_ERR_TOO_LARGE;      // 32-bit positions in a sequence
+    // the kernel for many rows stores 32 bytes at a time; asked of every call, so that it does not depend on the number of rows
+    if (reinterpret_cast<uintptr_t>(o) & 31) return BSA_ERR_ALIGNMENT;
     CachedParams p{};
     const int64_t group = q_heads / kv_heads;
     const int groups = row_groups(drafts * group);

@@ -41,7 +41,8 @@ enum {
     BSA_ERR_BAD_SHAPE = 4,      /* a size is negative, zero where it must not
                                    be, or not a multiple of the block size    */
     BSA_ERR_BAD_BLOCK = 5,      /* block (page) size is not 16, 32, 64 or 128 */
-    BSA_ERR_ALIGNMENT = 6,      /* a pointer is not 16-byte aligned           */
+    BSA_ERR_ALIGNMENT = 6,      /* a pointer is not 16-byte aligned (or 32,
+                                   where the entry point says so)             */
     BSA_ERR_WORKSPACE = 7,      /* workspace missing or too small             */
     BSA_ERR_LAUNCH = 8,         /* the CUDA runtime refused the launch        */
     BSA_ERR_DEVICE_TIMEOUT = 9, /* a bounded wait inside a kernel ran out; the
@@ -310,8 +311,8 @@ int bsa_cache_read(int dtype, int store, const int64_t* slots, int64_t tokens, c
  *                   reads key head h / (q_heads / kv_heads)
  *   keys, values, key_scales, value_scales, pages, page, dtype, store
  *                   the cache, as in bsa_cache_write
- *   o               [batch, drafts, q_heads, head_dim], contiguous; drafts that see
- *                   nothing, and those from counts[b] on, give 0
+ *   o               [batch, drafts, q_heads, head_dim], contiguous, 32-byte aligned;
+ *                   drafts that see nothing, and those from counts[b] on, give 0
  *   table           int32 [batch, table_width]: the pages of every sequence; only
  *                   entries before its length are read.  An id outside [0, pages)
  *                   leaves its keys out and is reported (BSA_ERR_BAD_SHAPE)

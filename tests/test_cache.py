@@ -116,6 +116,17 @@ def test_python_refusals_without_a_gpu():
         cached_attention(q, *cache, table, lengths)
 
 
+def test_cached_attention_output_on_32_bytes(lib):
+    """The kernel for many rows stores 32 bytes at a time; every output of this entry point is on 32, as the others'."""
+    f = lib.bsa_cached_attention
+    i, p, z = ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t
+    f.argtypes = [ctypes.c_int] * 2 + [p, i, i, i] + [p] * 10 + [i] * 11 + [ctypes.c_float, p, z, p, z, p]
+    for drafts in (1, 24):
+        for o in (16, 48, 40):
+            assert f(1, 0, 16, 1024, 1024, 128, 16, 16, None, None, o, 16, 16, None, None, None, 0, 0, 0, 1, drafts, 16, 4, 128, 4,
+                     64, 4, 1.0, 16, 1 << 40, 16, 256, None) == 6
+
+
 # ------------------------------------------------------------------------------------------------ GPU: write and read
 def _quantised(x):
     """e4m3 codes and fp32 scales by the definition, in the same order of fp32 operations (codes are compared exactly)."""
