@@ -414,6 +414,14 @@ torch::Tensor sparse_to_dense(torch::Tensor x, torch::Tensor row_blocks, int64_t
     return convert(false, x, row_blocks, rows, cols, block);
 }
 
+// Dual tensors do not require grad, so an op that is not (or not always) called through an autograd function would drop
+// their derivatives without a word.
+template <typename... Tensors>
+void refuse_forward_mode(const char* op, const Tensors&... tensors) {
+    const auto dual = [](const c10::optional<torch::Tensor>& t) { return t.has_value() && t->defined() && t->_fw_grad(0).defined(); };
+    TORCH_CHECK(!(dual(tensors) || ...), op, " has no forward-mode derivative");
+}
+
 // A paged cache as the bindings see it: [pages, heads, page, head_dim] twice, and for e4m3 the scales [pages, heads, page].
 struct Cache {
     int dtype, store;
@@ -472,6 +480,7 @@ void check_slots(const torch::Tensor& slots, const torch::Device& device) {
 // Keys and values of new tokens into the paged cache, in place.
 void cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torch::Tensor keys, torch::Tensor values,
                  c10::optional<torch::Tensor> key_scales, c10::optional<torch::Tensor> value_scales) {
+    refuse_forward_mode("cache_write", k, v, keys, values, key_scales, value_scales);
     TORCH_CHECK(k.dim() == 3 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() && k.device() == v.device(),
                 "k and v must share a shape [tokens, heads, head_dim], dtype and device");
     const Cache c = check_cache(keys, values, key_scales, value_scales, k.scalar_type(), k.device());
@@ -494,6 +503,7 @@ void cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torch::T
 std::tuple<torch::Tensor, torch::Tensor> cache_read(torch::Tensor slots, torch::Tensor keys, torch::Tensor values,
                                                     c10::optional<torch::Tensor> key_scales,
                                                     c10::optional<torch::Tensor> value_scales, at::ScalarType dtype) {
+    refuse_forward_mode("cache_read", keys, values, key_scales, value_scales);
     const Cache c = check_cache(keys, values, key_scales, value_scales, dtype, keys.device());
     check_slots(slots, keys.device());
     c10::cuda::CUDAGuard guard(keys.device());
@@ -515,6 +525,7 @@ torch::Tensor cached_attention(torch::Tensor q, torch::Tensor keys, torch::Tenso
                                torch::Tensor table, torch::Tensor lengths, c10::optional<torch::Tensor> counts,
                                c10::optional<torch::Tensor> tree, double scale, c10::optional<torch::Tensor> pattern,
                                int64_t pattern_block) {
+    refuse_forward_mode("cached_attention", q, keys, values, key_scales, value_scales);
     TORCH_CHECK(q.dim() == 4, "q must be [batch, drafts, heads, head_dim]");
     const Cache c = check_cache(keys, values, key_scales, value_scales, q.scalar_type(), q.device());
     const int64_t batch = q.size(0), drafts = q.size(1), heads = q.size(2);
@@ -702,6 +713,7 @@ public:
 
 torch::Tensor packed_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor offsets, double scale, bool causal,
                                bool check) {
+    refuse_forward_mode("packed_attention", q, k, v);
     const bool learns = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
     auto out = learns ? PackedAttention::apply(q, k, v, offsets, scale, causal, check)
                       : std::get<0>(packed_attention_forward(q, k, v, offsets, scale, causal, false));

@@ -18,6 +18,10 @@ A negative slot is skipped (written nowhere, read as zeros); one behind the
 cache's end is skipped too and reported through ``check_device_status``.  The
 non-negative slots of one write must differ: two tokens written to one slot
 leave a row that mixes both (``kernel.debug_checks`` raises instead).
+
+Serving only: no derivative passes through a cache.  Tokens that require grad may be
+written (their numbers are kept, as those of a detached tensor); a cache that requires
+grad is not read, and forward-mode derivatives are refused.
 """
 from typing import NamedTuple, Optional, Tuple
 
@@ -32,6 +36,12 @@ class Cache(NamedTuple):
     values: torch.Tensor
     key_scales: Optional[torch.Tensor] = None
     value_scales: Optional[torch.Tensor] = None
+
+
+def refuse_gradient(op: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Serving operators compute no gradient: asking for one is refused, not ignored."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("%s has no gradient: call it under torch.no_grad()" % op)
 
 
 def make_cache(pages: int, page: int, heads: int, head_dim: int, dtype: torch.dtype, device=None) -> Cache:
@@ -77,6 +87,7 @@ def cache_read(slots: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, ke
                dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values ``[tokens, heads, head_dim]`` at ``slots`` ``[tokens]``.  ``dtype``: type of the result,
     float16 or bfloat16 (a 16-bit cache's own by default, bfloat16 for float8_e4m3fn)."""
+    refuse_gradient("cache_read", keys, values, key_scales, value_scales)
     if dtype is None:
         dtype = torch.bfloat16 if keys.dtype == torch.float8_e4m3fn else keys.dtype
     k, v = kernel.sparse_ops.cache_read(slots, keys, values, key_scales, value_scales, dtype)

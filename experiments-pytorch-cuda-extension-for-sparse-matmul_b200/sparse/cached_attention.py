@@ -25,6 +25,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import kernel
+from .cache import refuse_gradient
 from .layout import SparseLayout
 
 
@@ -76,8 +77,7 @@ def cached_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     sequence has all drafts), ``tree`` int64 ``[batch, drafts]``.  Drafts from ``counts[b]`` on, and drafts that see
     nothing, give zeros.  Only table entries before a sequence's length are read; a page that is none of the cache's
     and a length behind the table's end leave those keys out and are reported by ``check_device_status``."""
-    if torch.is_grad_enabled() and (q.requires_grad or keys.requires_grad or values.requires_grad):
-        raise RuntimeError("cached_attention has no gradient: call it under torch.no_grad()")
+    refuse_gradient("cached_attention", q, keys, values, key_scales, value_scales)
     pattern, block = (None, 0) if layout is None else (_pattern(layout, q.device), layout.block)
     return kernel.check(kernel.sparse_ops.cached_attention(q, keys, values, key_scales, value_scales, table, lengths,
                                                            counts, tree, float(scale), pattern, block))

@@ -14,9 +14,9 @@ The forward keeps the output, what its rounding to 16 bits took (so that
 rowsum(dO o O) is exact to fp32) and the rows' log-sum-exp; the backward recomputes
 the probabilities on chip, by key tiles for dK and dV (summed over the heads
 that share a key head) and by query tiles for dQ, without atomics: gradients
-repeat bit for bit.  There is no second derivative.  A backward pass may be
-captured; it is refused while a graph recorded on the default stream still holds
-some of its leaves.
+repeat bit for bit.  There is no second derivative and no forward-mode one: both
+are refused.  A backward pass may be captured; it is refused while a graph recorded
+on the default stream still holds some of its leaves.
 """
 import torch
 

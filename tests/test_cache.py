@@ -127,6 +127,43 @@ def test_cached_attention_output_on_32_bytes(lib):
                      64, 4, 1.0, 16, 1 << 40, 16, 256, None) == 6
 
 
+def test_derivatives_that_the_cache_has_not_are_refused():
+    """Forward-mode derivatives (whose tensors do not require grad) and a cache that requires grad: refused, not dropped."""
+    import torch.autograd.forward_ad as fwd
+    from sparse import cache_read, cache_write, cached_attention, make_cache
+    k = torch.zeros(3, 2, 128, dtype=torch.float16)
+    slots = torch.arange(3)
+    q = torch.zeros(1, 1, 2, 128, dtype=torch.float16)
+    table, lengths = torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    plain, coded = make_cache(4, 64, 2, 128, torch.float16, device="cpu"), make_cache(4, 64, 2, 128, E4M3, device="cpu")
+    with fwd.dual_level(), torch.no_grad():
+        def dual(t):
+            return fwd.make_dual(t, torch.ones_like(t))
+        for a, b in ((dual(k), k), (k, dual(k))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                cache_write(a, b, slots, *plain)
+        for cache, side in ((plain, 0), (plain, 1), (coded, 2), (coded, 3)):
+            held = list(cache)
+            held[side] = dual(held[side])
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                cache_read(slots, *held, dtype=torch.float16)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                cached_attention(q, *held, table, lengths)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                cache_write(k, k, slots, *held)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            cached_attention(dual(q), *plain, table, lengths)
+    for cache, side in ((plain, 0), (plain, 1), (coded, 2), (coded, 3)):
+        held = list(cache)
+        held[side] = held[side].clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="no gradient"):
+            cache_read(slots, *held, dtype=torch.float16)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            cached_attention(q, *held, table, lengths)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            cache_read(slots, *held, dtype=torch.float16)
+
+
 # ------------------------------------------------------------------------------------------------ GPU: write and read
 def _quantised(x):
     """e4m3 codes and fp32 scales by the definition, in the same order of fp32 operations (codes are compared exactly)."""

@@ -51,6 +51,21 @@ def test_python_refusals_without_a_gpu():
         packed_attention(x, x, x, torch.tensor([0, 4], dtype=torch.int32))
 
 
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor does not require grad: its derivative would be dropped without a word."""
+    import torch.autograd.forward_ad as fwd
+    from sparse import packed_attention
+    x = torch.zeros(4, 2, 64, dtype=torch.float16)
+    offsets = torch.tensor([0, 4], dtype=torch.int32)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for args in ((dual, x, x), (x, dual, x), (x, x, dual), (dual, x.clone().requires_grad_(), x)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                packed_attention(*args, offsets)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                packed_attention(*args, offsets)
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 def _status():
     from sparse.kernel import sparse_ops
