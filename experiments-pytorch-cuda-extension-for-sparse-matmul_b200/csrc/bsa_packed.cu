@@ -25,6 +25,7 @@
 // 16,127 rows of 8 sequences, 16 / 4 heads x 128, bf16: 219 to 227 us, 930 to 960 TFLOP/s (194 us replayed on the
 // same inputs).  A pair of tiles takes 3100 cycles where the tensor pipe needs 2048: the chain of one tile (waiting for
 // its MMAs 1130 cycles, 400 until its maximum, 1330 of exponentials) is half hidden behind the other's.
+#include <climits>
 #include <type_traits>
 
 #include "bsa_packed_common.cuh"
@@ -152,7 +153,8 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
             }
             __syncwarp();
         };
-        bool more = true, listed = true;
+        bool more = true;
+        int behind = INT_MAX;                                   // the smallest rank found to lie behind the list's end
         int at = (int)blockIdx.x, next = 0;
         for (int round = 0; ok && more; ++round, at = next) {
             // The next item: the place of a CTA that has not started yet.  Asked for once this one's loads are out, about two
@@ -176,9 +178,9 @@ packed_forward_kernel(const PackedParams p, const __grid_constant__ CUtensorMap 
             };
             const int rank = at / head_items, head_item = at - rank * head_items, head0 = p.pair ? 2 * head_item : head_item;
             PackedItem found{0, 0, 0, 0};
-            if (listed) found = packed_locate(p.offsets, p.batch, p.rows, per_tile, rank, lane, p.status);
-            if (found.length == 0) {                            // behind the list's end, and so is everything after it
-                listed = false;
+            if (rank < behind) found = packed_locate(p.offsets, p.batch, p.rows, per_tile, rank, lane, p.status);
+            if (found.length == 0) {                            // behind the list's end, and so is every larger rank (a place
+                behind = min(behind, rank);                     // that is taken over later may have a smaller one)
                 take();
                 continue;
             }

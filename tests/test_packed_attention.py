@@ -469,3 +469,17 @@ def test_prompt_then_tokens_matches_the_whole():
     _status()
     over = (got.double() - reference[0]).abs() - bound[0]
     assert (over <= 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths,tail,hq,hk,dim", [([0] * 3000 + [5, 0, 300] + [0] * 2000 + [129], 0, 2, 1, 64),
+                                                    ([0] * 700 + [257] + [0] * 300, 140, 12, 12, 128)])
+def test_many_places_behind_the_end_of_the_list(lengths, tail, hq, hk, dim):
+    """The grid is an upper bound of the tiles: with thousands of empty sequences a CTA meets the list's end again and
+    again, and every tile that it is handed before or after is still made."""
+    q, k, v, do, offsets = _inputs(lengths, tail, hq, hk, dim, torch.bfloat16, 17)
+    got = _run(q, k, v, do, offsets, dim ** -0.5, True)
+    _status()
+    _check(got, _reference(q, k, v, do, lengths, dim ** -0.5, True))
+    for t in got:
+        assert (t[sum(lengths):] == 0).all()
