@@ -70,8 +70,8 @@ def cached_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
                      value_scales: Optional[torch.Tensor], table: torch.Tensor, lengths: torch.Tensor,
                      counts: Optional[torch.Tensor] = None, tree: Optional[torch.Tensor] = None, scale: float = 1.0,
                      layout: Optional[SparseLayout] = None) -> torch.Tensor:
-    """Attention of ``q [batch, drafts, heads, head_dim]`` (float16 or bfloat16, at most 64 drafts; ``heads`` a multiple
-    of the cache's) over the cache ``keys, values, key_scales, value_scales``; returns q's shape.
+    """Attention of ``q [batch, drafts, heads, head_dim]`` (float16 or bfloat16, at most 65536 sequences and 64 drafts;
+    ``heads`` a multiple of the cache's) over the cache ``keys, values, key_scales, value_scales``; returns q's shape.
 
     ``table`` int32 ``[batch, pages]``, ``lengths`` int32 ``[batch]``, ``counts`` int32 ``[batch]`` (default: every
     sequence has all drafts), ``tree`` int64 ``[batch, drafts]``.  Drafts from ``counts[b]`` on, and drafts that see

@@ -250,7 +250,8 @@ int bsa_attention_backward(int dtype, const void* q, const void* k, const void* 
  *                   rowsum(dout o O).  The forward writes both where a backward
  *                   follows; give NULL for both where none does.
  *   stats           scratch of rows * q_heads * 8 bytes, 16-byte aligned
- * BSA_DTYPE_F16 / BSA_DTYPE_BF16, head_dim 64 or 128.
+ * BSA_DTYPE_F16 / BSA_DTYPE_BF16, head_dim 64 or 128, at most 65536 sequences
+ * (BSA_ERR_TOO_LARGE): the time for finding the work grows with their square.
  */
 int bsa_packed_forward(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                        int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
@@ -328,7 +329,7 @@ int bsa_cache_read(int dtype, int store, const int64_t* slots, int64_t tokens, c
  *                   number of tokens before the drafts plus that of its ancestors.
  *   scratch         bsa_cached_attention_scratch() bytes, 16-byte aligned, of this
  *                   call alone until it is done
- * drafts <= 64.
+ * drafts <= 64, batch <= 65536 (BSA_ERR_TOO_LARGE).
  */
 size_t bsa_cached_attention_scratch(int64_t drafts, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
 int bsa_cached_attention(int dtype, int store, const void* q, int64_t q_batch_stride, int64_t q_draft_stride,

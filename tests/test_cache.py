@@ -74,6 +74,18 @@ def test_cached_attention_validation_codes(lib):
     assert call(batch=0) == 0
 
 
+def test_cached_attention_number_of_sequences(lib):
+    """The join's time grows with the square of the number of sequences: one that would hold the device is refused."""
+    f = lib.bsa_cached_attention
+    i, p, z = ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t
+    f.argtypes = [ctypes.c_int] * 2 + [p, i, i, i] + [p] * 10 + [i] * 11 + [ctypes.c_float, p, z, p, z, p]
+
+    def call(batch):                                       # (without queries: the sizes are looked at first)
+        return f(1, 0, None, 1024, 1024, 128, 16, 16, None, None, 32, 16, 16, None, None, None, 0, 0, 0, batch, 1, 8, 4, 128, 4, 64, 4,
+                 1.0, 16, 1 << 40, 16, 256, None)
+    assert call(65537) == 10 and call(2 ** 24) == 10 and call(65536) == 1
+
+
 def test_tree_words_and_their_refusals():
     from sparse import tree_words
     assert tree_words([[-1, 0, 0, 2, -1]]).tolist() == [[0b1, 0b11, 0b101, 0b1101, 0b10000]]

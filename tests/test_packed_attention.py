@@ -44,6 +44,23 @@ def test_packed_validation_codes():
     assert back(dk=48) == 6 and back(stats_bytes=10 * 8 * 8 - 1) == 7 and back(rows=0) == 0
 
 
+def test_packed_number_of_sequences():
+    """Finding the work takes time that grows with the square of the number of sequences: one that would hold the device
+    for minutes is refused."""
+    path = os.path.join(PKG, "libbsa_b200.so")
+    if not os.path.exists(path):
+        pytest.skip("kernel library not built")
+    lib = ctypes.CDLL(path)
+    i, p, z = ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t
+    lib.bsa_packed_forward.argtypes = [ctypes.c_int] + [p, i, i] * 3 + [p, p, p, p] + [i] * 5 + [ctypes.c_float, ctypes.c_int, p, z, p]
+    lib.bsa_packed_backward.argtypes = [ctypes.c_int] + [p, i, i] * 3 + [p, p, p, i, i] + [p] * 5 + [i] * 5 + [ctypes.c_float, ctypes.c_int, p, z, p, z, p]
+    for batch, code in ((65537, 10), (2 ** 24, 10), (65536, 1)):       # (without queries: the sizes are looked at first)
+        assert lib.bsa_packed_forward(1, None, 1024, 128, 32, 512, 128, 32, 512, 128, 32, None, None, 32, 10, batch, 8, 4, 128, 1.0, 1,
+                                      16, 256, None) == code
+        assert lib.bsa_packed_backward(1, None, 1024, 128, 32, 512, 128, 32, 512, 128, 32, 32, 32, 1024, 128, 32, 32, 32, 32, 32, 10,
+                                       batch, 8, 4, 128, 1.0, 1, 32, 1 << 20, 16, 256, None) == code
+
+
 def test_python_refusals_without_a_gpu():
     from sparse import packed_attention
     x = torch.zeros(4, 2, 64, dtype=torch.float16)
