@@ -62,12 +62,14 @@ def make_cache(pages: int, page: int, heads: int, head_dim: int, dtype: torch.dt
 
 def cache_slots(table: torch.Tensor, sequences: torch.Tensor, positions: torch.Tensor, page: int) -> torch.Tensor:
     """Slots (int64) of ``positions`` of ``sequences`` (broadcast together, flattened): sequence ``s`` has its pages in
-    row ``s`` of ``table`` ``[sequences, pages]``.  -1 where the position is negative or behind the table's end, or
-    where the table holds a negative page."""
+    row ``s`` of ``table`` ``[sequences, pages]``.  -1 where the sequence is none of the table's, the position is negative
+    or behind the table's end, or the table holds a negative page."""
     sequences, positions = torch.broadcast_tensors(sequences, positions)
     sequences, positions = sequences.reshape(-1).long(), positions.reshape(-1).long()
-    inside = (positions >= 0) & (positions < table.size(1) * page)
-    held = table.long()[sequences, torch.where(inside, positions, 0) // page]
+    inside = (sequences >= 0) & (sequences < table.size(0)) & (positions >= 0) & (positions < table.size(1) * page)
+    if table.numel() == 0:
+        return torch.full_like(positions, -1)
+    held = table.long()[torch.where(inside, sequences, 0), torch.where(inside, positions, 0) // page]
     return torch.where(inside & (held >= 0), held * page + positions % page, -1)
 
 

@@ -139,6 +139,16 @@ def test_cached_attention_output_on_32_bytes(lib):
                      64, 4, 1.0, 16, 1 << 40, 16, 256, None) == 6
 
 
+def test_cache_slots_of_sequences_that_are_none():
+    """A sequence outside the table has no slots: a negative number does not count from the table's end."""
+    from sparse import cache_slots
+    table = torch.tensor([[5, 2], [7, 3]], dtype=torch.int32)
+    got = cache_slots(table, torch.tensor([-1, 0, 1, 2, 2 ** 40, -3]), torch.tensor([0, 1, 17, 0, 5, 1]), 16)
+    assert got.tolist() == [-1, 81, 49, -1, -1, -1]
+    assert cache_slots(table[:, :0], torch.tensor([0, 1]), torch.tensor([0, 1]), 16).tolist() == [-1, -1]
+    assert cache_slots(table[:0], torch.tensor([0, 1]), torch.tensor([0, 1]), 16).tolist() == [-1, -1]
+
+
 def test_derivatives_that_the_cache_has_not_are_refused():
     """Forward-mode derivatives (whose tensors do not require grad) and a cache that requires grad: refused, not dropped."""
     import torch.autograd.forward_ad as fwd
