@@ -815,3 +815,22 @@ def test_places_that_were_never_written_count_as_zeros(drafts):
         assert ((got - want).abs() <= off * held[1].abs().amax()).all()
         assert (got[1] == 0).all()
     _status()
+
+
+# ------------------------------------------------------------------------------------------------ layouts
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", ["same", "e4m3"])
+@pytest.mark.parametrize("block,page,dim,group,drafts,tree", [(32, 64, 64, 2, 1, False), (128, 16, 128, 4, 9, True),
+                                                              (64, 32, 64, 3, 11, False), (64, 128, 64, 5, 15, True),
+                                                              (16, 16, 128, 2, 64, True)])
+def test_cached_attention_with_a_layout_over_both_caches_and_many_rows(store, block, page, dim, group, drafts, tree):
+    """One row group to several row tiles (drafts x group of 2 to 128), drafts on both sides of a block's border."""
+    from sparse import SparseLayout
+    lengths = [700, 129, 64, 9, 0, 2 * block + 5]
+    counts = [min(n, drafts) for n in lengths]
+    pattern = (torch.rand(6 * 128 // block, 6 * 128 // block, generator=torch.Generator().manual_seed(block)) < 0.4).to(torch.uint8)
+    pattern[2] = 0                                         # a block row without blocks: its rows see nothing
+    case = _Case(torch.float16, store, dim, page, 2, group, drafts, lengths, counts, tree=tree, seed=block)
+    got = case.call(layout=SparseLayout(pattern, block=block))
+    _status()
+    _check(got, case.reference(pattern, block))
