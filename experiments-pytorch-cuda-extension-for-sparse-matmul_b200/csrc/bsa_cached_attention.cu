@@ -357,19 +357,31 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             const int key0 = tile * kTileKeys + base, tile_end = (tile + 1) * kTileKeys;
             const bool all_loaded = loaded == (1u << (kTileKeys >> min(p.page_shift, 6))) - 1u;
             const bool masked = tile_end > prefix || !all_loaded || p.pattern != nullptr;
-            // The step's 32 keys as bits: what is there, and below what each of the two rows sees.  (Written out per element this
-            // was most of the kernel's code, and a short sequence, all of whose steps are masked, waited for it to be fetched.)
-            uint32_t there = 0xffffffffu;
+            // The step's 32 keys as bits: what each of the two rows sees, and what any row of the warp does: the other keys may
+            // hold anything.  (Written out per element this was most of the kernel's code, and a short sequence, all of whose
+            // steps are masked, waited for it to be fetched.)
+            uint32_t seen[2] = {0xffffffffu, 0xffffffffu}, used = 0xffffffffu;
             if (masked) {
-                const int shift = min(p.page_shift, 6);
-                there = shift >= 5 ? (loaded >> (base >> shift) & 1u ? 0xffffffffu : 0u)
-                                   : ((loaded >> (base >> 4) & 1u ? 0xffffu : 0u) | (loaded >> ((base >> 4) + 1) & 1u ? 0xffff0000u : 0u));
+                const int shift = min(p.page_shift, 6), d = key0 - prefix;
+                uint32_t there = shift >= 5 ? (loaded >> (base >> shift) & 1u ? 0xffffffffu : 0u)
+                                            : ((loaded >> (base >> 4) & 1u ? 0xffffu : 0u) | (loaded >> ((base >> 4) + 1) & 1u ? 0xffff0000u : 0u));
                 there &= below(length - key0);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const uint32_t drafts = d >= 64 || d <= -32 ? 0u : (d >= 0 ? (uint32_t)(sees[r] >> d) : (uint32_t)sees[r] << -d);
+                    seen[r] = row_on[r] ? there & (below(-d) | drafts) : 0u;
+                    if (p.pattern)
+                        seen[r] = row_block[r] < 0 || row_block[r] >= p.pattern_rows ? 0u :
+                            seen[r] & in_pattern(p.pattern + (int64_t)row_block[r] * p.pattern_cols, p.pattern_cols, p.pattern_shift,
+                                                 p.tree ? p.tree + (int64_t)b * p.drafts : nullptr, key0, prefix, seen[r]);
+                }
+                __syncwarp();
+                used = __reduce_or_sync(0xffffffffu, seen[0] | seen[1]);
             }
             // e4m3: a lane brings the scales of one key, the warp shares them (the key's, and the value's over r)
             if (kE4m3) {
                 const float* scales = reinterpret_cast<const float*>(scale_smem + stage * S::kScaleBytes) + base + lane;
-                const float sv = there >> lane & 1u ? scales[kTileKeys] : 0.0f;
+                const float sv = used >> lane & 1u ? scales[kTileKeys] : 0.0f;
                 const uint32_t size = __float_as_uint(sv) & 0x7fffffffu;
                 const bool finite = size < 0x7f800000u;
                 if (__any_sync(0xffffffffu, finite && size >= r_bits + 4 * kExponent)) {
@@ -433,28 +445,16 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
                     for (int e = 0; e < 4; ++e) s[n][e] *= row_scale[e >> 1];
                 }
             }
-            uint32_t keep[kNT];                             // per n-tile: which of this thread's two keys are really there
+            uint32_t keep[kNT];                             // per n-tile: which of this thread's two keys are used
             if (masked) {
-                const int d = key0 - prefix;
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const uint32_t drafts = d >= 64 || d <= -32 ? 0u : (d >= 0 ? (uint32_t)(sees[r] >> d) : (uint32_t)sees[r] << -d);
-                    uint32_t seen = row_on[r] ? there & (below(-d) | drafts) : 0u;
-                    if (p.pattern)
-                        seen = row_block[r] < 0 || row_block[r] >= p.pattern_rows ? 0u :
-                            seen & in_pattern(p.pattern + (int64_t)row_block[r] * p.pattern_cols, p.pattern_cols, p.pattern_shift,
-                                              p.tree ? p.tree + (int64_t)b * p.drafts : nullptr, key0, prefix, seen);
-                    seen >>= 2 * c;
+                for (int n = 0; n < kNT; ++n) {
+                    const int at = 8 * n + 2 * c;
+                    keep[n] = (used >> at & 1u ? 0x0000ffffu : 0u) | (used >> (at + 1) & 1u ? 0xffff0000u : 0u);
 #pragma unroll
-                    for (int n = 0; n < kNT; ++n)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            if (!(seen >> (8 * n + e) & 1u)) s[n][2 * r + e] = -INFINITY;
+                    for (int e = 0; e < 4; ++e)
+                        if (!(seen[e >> 1] >> (at + (e & 1)) & 1u)) s[n][e] = -INFINITY;
                 }
-                there >>= 2 * c;
-#pragma unroll
-                for (int n = 0; n < kNT; ++n)
-                    keep[n] = (there >> (8 * n) & 1u ? 0x0000ffffu : 0u) | (there >> (8 * n + 1) & 1u ? 0xffff0000u : 0u);
             }
             // The running maximum is raised only where a score exceeds it by more than 8 (units of log2): P stays below
             // 2^8, and O and l carry the same factor whatever it is.
@@ -504,7 +504,7 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
                     uint32_t vf[4];
                     // (a is even, so the chunk's number goes into the swizzled address as an exclusive or)
                     ldsm_x4_trans((rows16 ^ (uint32_t)((a & 7) << 4)) + (uint32_t)((a >> 3) * (kTileKeys * 128)), vf);
-                    if (masked) {                           // what is not there may be anything, a NaN too
+                    if (masked) {                           // what no row sees may be anything, a NaN too
                         vf[0] &= keep[2 * ks]; vf[1] &= keep[2 * ks + 1];
                         vf[2] &= keep[2 * ks]; vf[3] &= keep[2 * ks + 1];
                     }

@@ -834,3 +834,34 @@ def test_cached_attention_with_a_layout_over_both_caches_and_many_rows(store, bl
     got = case.call(layout=SparseLayout(pattern, block=block))
     _status()
     _check(got, case.reference(pattern, block))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", ["same", "e4m3"])
+@pytest.mark.parametrize("group,drafts", [(2, 1), (4, 5), (3, 22)])
+def test_numbers_of_blocks_outside_the_layout_are_not_used(store, group, drafts):
+    """Keys and values of places that no draft of a sequence sees under the layout may be NaN."""
+    from sparse import SparseLayout
+    block, page = 32, 16
+    lengths = [500, 90, 33]
+    gen = torch.Generator().manual_seed(5)
+    pattern = (torch.rand(16, 16, generator=gen) < 0.4).to(torch.uint8) | torch.eye(16, dtype=torch.uint8)
+    case = _Case(torch.bfloat16, store, 64, page, 2, group, drafts, lengths, tree=drafts > 5, seed=6)
+    reference = case.reference(pattern, block)
+    hidden = 0
+    for b, n in enumerate(lengths):
+        for j in (~case.seen(b, pattern, block).any(0)).nonzero()[:, 0].tolist():
+            at = (int(case.table[b, j // page]), slice(None), j % page)
+            hidden += 1
+            for t in (case.keys, case.values):
+                if store == "e4m3":
+                    t.view(torch.uint8)[at] = 0x7f
+                else:
+                    t[at] = math.nan
+            if store == "e4m3":
+                case.key_scales[at] = math.nan
+                case.value_scales[at] = math.inf
+    assert hidden > 100
+    got = case.call(layout=SparseLayout(pattern, block=block))
+    _status()
+    _check(got, reference)
