@@ -117,6 +117,9 @@ __device__ __forceinline__ uint32_t chunk_offset(int row, int chunk) {
     return (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
 }
 
+// How many other drafts a draft sees (its own bit may be set or not).
+__device__ __forceinline__ int ancestors(uint64_t word, int draft) { return __popcll(word & ~(1ull << draft)); }
+
 // Of 32 keys from key0 on, those (of `wanted`) whose block is in the layout, seen from block row `row`.  Whole blocks before
 // the drafts are one lookup per 16 keys; a draft stands behind the prefix and its ancestors.
 // (`at`: the row of the pattern; `tree`: the sequence's words, or null)
@@ -135,7 +138,7 @@ __device__ __noinline__ uint32_t in_pattern(const uint8_t* at, int cols, int shi
         int place = key;
         if (draft >= 0) {
             const uint64_t w = tree ? (uint64_t)tree[draft] : ~0ull >> (63 - draft);
-            place = max(prefix, 0) + max(__popcll(w) - 1, 0);
+            place = max(prefix, 0) + ancestors(w, draft);
         }
         const int block = place >> shift;
         if (block < cols && at[block]) bits |= 1u << k;
@@ -296,8 +299,8 @@ cached_attention_kernel(const CachedParams p, const __grid_constant__ CUtensorMa
             row_block[r] = -1;
             if (row_on[r]) {
                 sees[r] = p.tree ? (uint64_t)p.tree[(int64_t)b * p.drafts + draft] : ~0ull >> (63 - draft);
-                // a draft stands behind the prefix and its ancestors: its depth is the number of those
-                if (p.pattern) row_block[r] = (max(length - count, 0) + max(__popcll(sees[r]) - 1, 0)) >> p.pattern_shift;
+                // a draft stands behind the prefix and its ancestors
+                if (p.pattern) row_block[r] = (max(length - count, 0) + ancestors(sees[r], draft)) >> p.pattern_shift;
             }
         }
     };

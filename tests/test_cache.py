@@ -865,3 +865,35 @@ def test_numbers_of_blocks_outside_the_layout_are_not_used(store, group, drafts)
     got = case.call(layout=SparseLayout(pattern, block=block))
     _status()
     _check(got, reference)
+
+
+class _Blind(_Case):
+    """Drafts that do not see themselves (bit i of word i is not set): their ancestors are all that they see."""
+
+    def seen(self, b, pattern=None, block=1):
+        n, c = self.lengths[b], self.drafts if self.counts is None else self.counts[b]
+        words = [w & (1 << 64) - 1 for w in self.tree[b].tolist()]
+        place = [max(n - c, 0) + bin(w & ~(1 << i)).count("1") for i, w in enumerate(words)]
+        seen = torch.zeros(self.drafts, n, dtype=torch.bool)
+        for i in range(min(c, self.drafts)):
+            for j in range(n):
+                d = j - (n - c)
+                row, col = place[i] // block, (j if d < 0 else place[d]) // block
+                seen[i, j] = (d < 0 or bool(words[i] >> d & 1)) and (pattern is None or bool(pattern[row, col]))
+        return seen
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drafts,group", [(5, 2), (20, 3)])
+def test_position_of_a_draft_that_does_not_see_itself(drafts, group):
+    """It stands behind its ancestors as any other does: on the borders of small blocks one place decides."""
+    from sparse import SparseLayout
+    block = 16
+    lengths = [16 * 7 + 3, 16 * 3 + drafts, 16 * 5 + drafts - 1, 16 * 4 + drafts - 2]
+    pattern = (torch.rand(12, 12, generator=torch.Generator().manual_seed(3)) < 0.5).to(torch.uint8)
+    case = _Blind(torch.float16, "same", 64, 16, 2, group, drafts, lengths, tree=True, seed=9)
+    for i in range(0, drafts, 2):
+        case.tree[:, i] &= ~(1 << i)
+    got = case.call(layout=SparseLayout(pattern, block=block))
+    _status()
+    _check(got, case.reference(pattern, block))
