@@ -31,9 +31,14 @@
 // The weights are rounded to the products' 16-bit type (half a step: relative 2^-8 in bf16, 2^-11 in fp16), l, m and O are
 // fp32.
 //
-// 32 sequences of 1 to 8192 tokens, 8 heads x 128, e4m3 (94 MB): 32.9 us, 2.9 TB/s; bound by the latency of a warp's
+// 32 sequences of 1 to 8192 tokens, 8 heads x 128, e4m3 (94 MB): 32.8 us, 2.9 TB/s; bound by the latency of a warp's
 // step of 32 keys (2100 cycles with 2 consumer warps per scheduler) and what begins a share (2,800 cycles) and ends it
-// (2,200 to 5,400).  One token over 391: 10.3 us a call, 8.8 in a graph.
+// (2,200 to 5,400).  One token over 391: 10.3 us a call, 9.2 in a graph.
+//
+// A layout takes keys away from the softmax, not from the work: every page is brought and multiplied all the same, and a
+// step looks its blocks up besides.  One sequence of 32,768 tokens, 4 heads x 128, whose last row keeps 5 of 512 blocks,
+// 16 bits: one token 38.9 us with and without; 16 tokens of 16 query heads 65.4 us here, 38.9 without it in the kernel for
+// many rows, which takes no layout; e4m3 36.9 and 32.8, 67.6 and 53.2.
 #include <algorithm>
 #include <type_traits>
 
@@ -44,8 +49,9 @@ namespace {
 
 constexpr int kTileKeys = 64;
 constexpr int kConsumers = 4;                   // warps
-constexpr int kBegin = 6;                       // what beginning and ending a (sequence, head) costs a CTA, in tiles (batch of
-                                                // 32 of 1 to 8192 tokens: with 3 47.6 us, 5 37.4, 7 36.9, 10 38.5)
+constexpr int kBegin = 6;                       // what beginning and ending a (sequence, head) costs a CTA, in tiles.  Found on one
+                                                // batch (32 of 1 to 8192 tokens, e4m3: with 3 37.1 us, 5 32.5, 6 32.8, 7 32.9,
+                                                // 10 34.8) and used for every type; one token of one sequence does not feel it
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kExponent = 1u << 23;        // one step of an fp32 number's exponent
 // Query rows of a key head above which a 16-bit cache goes to the tcgen05 kernel.  8 x 4000 tokens of 4 heads x 128: 32 rows

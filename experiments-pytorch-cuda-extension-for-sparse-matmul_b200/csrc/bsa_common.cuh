@@ -76,8 +76,5 @@ bool attention_supports(int dtype, int64_t head_dim, int block);
 // argument checks that every entry point over a paged cache makes (types, scales, page and head sizes)
 int check_cache(int dtype, int store, const float* key_scales, const float* value_scales, int64_t pages, int64_t heads,
                 int64_t page, int64_t dim);
-// argument checks that every entry point over a paged cache makes (types, scales, page and head sizes)
-int check_cache(int dtype, int store, const float* key_scales, const float* value_scales, int64_t pages, int64_t heads,
-                int64_t page, int64_t dim);
 
 }  // namespace bsa
