@@ -16,10 +16,10 @@ key at position j is seen from position i only where the layout has the block
 (i // block, j // block).  A draft's position is the number of tokens before
 the drafts plus the number of its ancestors.
 
-Serving only: there is no gradient.  A NaN or an infinity among the values that
-one draft of a sequence sees may reach all of that sequence's rows, never another
-sequence's.  What lies behind a sequence's length, and what the layout hides from
-all of its drafts, is never used.
+Serving only: there is no gradient.  A NaN or an infinity among the values of a
+sequence's drafts, or of a place that one of them sees, may reach all of that
+sequence's rows, never another sequence's.  What lies behind a sequence's length,
+and what the layout hides from all of its drafts, is never used.
 """
 from typing import Optional, Sequence
 

@@ -29,7 +29,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     dimension 64 or 128, ``heads`` a multiple of ``kv_heads``; views of one projection are read in place).
 
     ``offsets`` int32 ``[sequences + 1]`` on q's device: sequence ``b`` is the rows ``offsets[b] .. offsets[b + 1] - 1``
-    (it may be empty; at most 65536 sequences); ``offsets[0]`` is 0.  Rows behind the last sequence give zeros, and zero gradients.  Offsets that
-    decrease or pass the last row are reported by ``check_device_status``.  A NaN or an infinity reaches rows of its own
-    sequence only."""
+    (it may be empty; at most 65536 sequences); ``offsets[0]`` is 0.  Rows behind the last sequence give zeros, and zero
+    gradients.  Offsets that decrease or pass the last row are reported by ``check_device_status``.  A NaN or an infinity
+    reaches rows of its own sequence only."""
     return kernel.sparse_ops.packed_attention(q, k, v, offsets, float(scale), bool(causal), kernel.debug_checks)

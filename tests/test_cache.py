@@ -897,3 +897,18 @@ def test_position_of_a_draft_that_does_not_see_itself(drafts, group):
     got = case.call(layout=SparseLayout(pattern, block=block))
     _status()
     _check(got, case.reference(pattern, block))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,drafts", [(1, 1), (40, 1)])
+def test_as_many_sequences_as_there_may_be(group, drafts):
+    """65536 sequences of one token: every row is its value, bit for bit."""
+    from sparse import cached_attention
+    n, dim, page = 65536, 64, 16
+    k, v = (_normal((n, 1, page, dim), i, torch.float16).cuda() for i in (1, 2))
+    q = _normal((n, drafts, group, dim), 3, torch.float16).cuda()
+    table = torch.randperm(n, generator=torch.Generator().manual_seed(4)).to(torch.int32)[:, None].cuda()
+    lengths = torch.ones(n, dtype=torch.int32, device="cuda")
+    got = cached_attention(q, k, v, None, None, table, lengths, scale=0.125)
+    _status()
+    assert torch.equal(got, v[table[:, 0].long(), :, :1].expand(-1, -1, group, -1))

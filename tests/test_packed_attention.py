@@ -500,3 +500,17 @@ def test_many_places_behind_the_end_of_the_list(lengths, tail, hq, hk, dim):
     _check(got, _reference(q, k, v, do, lengths, dim ** -0.5, True))
     for t in got:
         assert (t[sum(lengths):] == 0).all()
+
+
+@pytest.mark.gpu
+def test_as_many_sequences_as_there_may_be():
+    """65536 sequences of one row: a row's only weight is 1, so its output is its value and dV is dO, bit for bit."""
+    n, dim, scale = 65536, 64, 0.125
+    q, k, v, do, offsets = _inputs([1] * n, 0, 1, 1, dim, torch.float16, 19)
+    out, dq, dk, dv = _run(q, k, v, do, offsets, scale, True)
+    _status()
+    assert torch.equal(out.cpu(), v) and torch.equal(dv.cpu(), do)
+    # dP and delta are the same sum in another order: 2 dim steps of its magnitudes, and once rounded to fp16
+    off = 2 * dim * 2.0 ** -24 * (do.double().abs() * v.double().abs()).sum(-1, keepdim=True) + 2.0 ** -25
+    assert (dq.double().cpu().abs() <= scale * 1.01 * off * k.double().abs() + 2.0 ** -25).all()
+    assert (dk.double().cpu().abs() <= scale * 1.01 * off * q.double().abs() + 2.0 ** -25).all()
